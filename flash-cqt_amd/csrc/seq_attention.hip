@@ -109,7 +109,7 @@ int run(Chunks& a, const Plan& p, bool only_states, int slope, int64_t batch, in
     a.segments = p.segments;
     a.chunks = int32_t(p.tokens / tokens_of_chunk(dtype));
     a.spread = !only_states && !a.reduce && spreads(p, batch, heads, a.group);
-    Launch l{p.kd, p.waves, only_states, a.last.data != nullptr, slope,
+    Launch l{p.kd, p.waves, only_states, slope,
              dim3(p.segments, a.spread ? heads * a.group : heads, uint32_t(batch)), stream};
     if (dtype == FCQT_F32) launch_f32(a, l);
     else if (dtype == FCQT_BF16) launch_bf16(a, l);

@@ -22,9 +22,10 @@
 // of the next product wants once the products' inner index is taken in the order 0-3, 8-11 | 4-7, 12-15, which the
 // tiles of q and k are stored in. Operands whose inner index is the token are read with the transposing LDS load.
 //
-// Precision: bf16 inputs are exact operands; what is computed (P, the state, the decayed v) is split into bf16 planes
-// whose sum is the fp32 value to 16 (two planes) or 24 bits (three). fp16 inputs are two planes, fp32 ones three: six
-// bf16 products for one fp32 product take 192 cycles where v_mfma_f32_32x32x2_f32 takes 512.
+// Precision: bf16 inputs are exact operands, fp16 ones two planes, and fp32 ones and what is computed (P, the state, the
+// decayed v) three bf16 planes whose sum is the fp32 value: six bf16 products for one fp32 product take 192 cycles where
+// v_mfma_f32_32x32x2_f32 takes 512. (Two planes for what 16-bit outputs are made of would leave 2^-17 of each operand, and
+// o 1.3e-6 of its size away from its value before the rounding, where three leave 2e-7.)
 //
 // What bounds it: 1 x 65537 bf16 tokens of 16 heads, 128 wide, take 290 us in the main kernel (1.07 GB, 3.7 TB/s; its
 // loads alone 182 us, its instructions alone 290) after 127 us for the segments' own states (0.54 GB, 4.2 TB/s): about
@@ -128,15 +129,17 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&y)[N]) {
     }
 }
 
-// acc += a b over the planes whose product counts: those of order kOrder and below, the small ones first
-template <int kOrder, int NA, int NB>
+// acc += a b over the planes whose product counts (of order two and below: the others are under 2^-24), the small ones first
+template <int NA, int NB>
 __device__ __forceinline__ void multiply(f32x16& acc, const bf16x8 (&a)[NA], const bf16x8 (&b)[NB]) {
 #pragma unroll
-    for (int order = kOrder; order >= 0; --order)
+    for (int order = 2; order >= 0; --order)
 #pragma unroll
         for (int i = 0; i < NA; ++i)
             if (order - i >= 0 && order - i < NB) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[order - i], acc, 0, 0, 0);
 }
+
+constexpr int kPlanes = 3;          // of what is computed
 
 // eight input elements as they lie in memory
 template <class T>
@@ -173,10 +176,10 @@ __device__ __forceinline__ float power(float g, int n) {
     return fabsf(x) < 100.0f ? fmaf(y, fmaf(g, float(n), -x), y) : y;
 }
 
-// PP, PS, PU: planes of P, of the state as an operand, of the decayed v. kStates: states alone, no output. kSlope: with
-// the slope's terms (1 of dq, 2 of dk). kWaves: waves of a SIMD that the registers are shared among.
-template <class T, int KD, int NW, int PP, int PS, int PU, bool kStates, int kSlope, int kWaves>
-__global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
+// kStates: states alone, no output. kSlope: with the slope's terms (1 of dq, 2 of dk). Its registers are shared among two
+// waves of a SIMD.
+template <class T, int KD, int NW, bool kStates, int kSlope>
+__global__ __launch_bounds__(64 * NW, 2) void k_chunks(Chunks a) {
     constexpr int NI = Planes<T>::n;
     using Z = Tile<NI, KD, NW, kSlope == 1>;
     constexpr int C = Z::C, NT = Z::threads, IT = C / 32, MT = KD / 32, TILES = IT * (IT + 1) / 2;
@@ -479,7 +482,7 @@ __global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
                     if constexpr (kSlope == 1 && inter) {
                         if (crosses && kAhead == 1) load_z(s);
                     }
-                    bf16x8 Q[IT][NI], K[NI], X[PS];
+                    bf16x8 Q[IT][NI], K[NI], X[kPlanes];
 #pragma unroll
                     for (int i = 0; i < IT; ++i)
 #pragma unroll
@@ -488,16 +491,16 @@ __global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
                         float x[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) x[e] = S[s / 2][8 * (s % 2) + e];
-                        split<PS>(x, X);
+                        split<kPlanes>(x, X);
 #pragma unroll
-                        for (int i = 0; i < IT; ++i) multiply<PS - 1>(O[i], X, Q[i]);
+                        for (int i = 0; i < IT; ++i) multiply(O[i], X, Q[i]);
                     }
 #pragma unroll
                     for (int j = 0; j < (kLater ? 1 : IT); ++j) {
 #pragma unroll
                         for (int p = 0; p < NI; ++p) K[p] = *reinterpret_cast<const bf16x8*>(kat + p * Z::kplane + j * 32 * Z::krow + s * 16);
 #pragma unroll
-                        for (int i = j; i < IT; ++i) multiply<2>(A[i * (i + 1) / 2 + j], K, Q[i]);
+                        for (int i = j; i < IT; ++i) multiply(A[i * (i + 1) / 2 + j], K, Q[i]);
                     }
                     if constexpr (kSlope == 1 && inter) {
                         if (crosses) {
@@ -559,7 +562,7 @@ __global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
                             Q[p] = *reinterpret_cast<const bf16x8*>(qat + p * Z::kplane + j * 32 * Z::krow + s * 16);
                             K[p] = *reinterpret_cast<const bf16x8*>(kat + p * Z::kplane + j * 32 * Z::krow + s * 16);
                         }
-                        multiply<2>(A[TILES - 1], K, Q);
+                        multiply(A[TILES - 1], K, Q);
                         if (s % kFence == kFence - 1) fence();
                     }
                 }
@@ -581,7 +584,7 @@ __global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
                             rows_of(w[i * kw], s, W);
 #pragma unroll
                             for (int p = 0; p < NI; ++p) R[p] = *reinterpret_cast<const bf16x8*>(vs + hidden(col) * Z::vrow + wave * 32 + hidden(half) * 8 + p * Z::vplane + j * 32 * Z::vrow + s * 16);
-                            multiply<2>(B, R, W);
+                            multiply(B, R, W);
                         }
                         fence();
                     }
@@ -589,11 +592,11 @@ __global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         float x[8];
-                        bf16x8 P[PP];
+                        bf16x8 P[kPlanes];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) x[e] = A[i * (i + 1) / 2 + j][8 * s + e] * near[x0 + 8 * (2 * s + e / 4) + e % 4];
-                        split<PP>(x, P);
-                        multiply<PP - 1>(O[i], V[s], P);
+                        split<kPlanes>(x, P);
+                        multiply(O[i], V[s], P);
                         if constexpr (kSlope == 1) {
                             const float d = float(hidden(i * 32 + col - j * 32 - 4 * half));
 #pragma unroll
@@ -608,7 +611,7 @@ __global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 float x[8];
-                bf16x8 W[PU];
+                bf16x8 W[kPlanes];
                 const f32x4 f0 = *reinterpret_cast<const f32x4*>(&left[j * 32 + s * 16 + 4 * half]);
                 const f32x4 f1 = *reinterpret_cast<const f32x4*>(&left[j * 32 + s * 16 + 8 + 4 * half]);
 #pragma unroll
@@ -618,14 +621,14 @@ __global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
                     for (int p = NI - 2; p >= 0; --p) v += float(V[s][p][e]);
                     x[e] = v * (e < 4 ? f0[e % 4] : f1[e % 4]);
                 }
-                split<PU>(x, W);
+                split<kPlanes>(x, W);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     bf16x8 K[NI];
 #pragma unroll
                     for (int p = 0; p < NI; ++p)
                         K[p] = transposed(ktr + p * Z::kplane + (j * 32 + s * 16) * Z::krow + m * 32, 8 * Z::krow);
-                    multiply<PU - 1>(S[m], K, W);
+                    multiply(S[m], K, W);
                     if (m % 2) fence();
                 }
                 fence();
@@ -687,24 +690,18 @@ __global__ __launch_bounds__(64 * NW, kWaves) void k_chunks(Chunks a) {
 // Which kernel, and over what. grid: segments, key heads (or query heads), rows.
 struct Launch {
     int kd, waves;                  // the kernel's sizes: 32, 64 or 128, 2 or 4
-    bool states, last;              // states alone; with the last state
+    bool states;                    // states alone
     int slope;                      // kSlope
     dim3 grid;
     hipStream_t stream;
 };
 
-// The last number is the waves of a SIMD that its registers are shared among.
 template <class T, int KD, int NW>
 void launch_sized(const Chunks& a, const Launch& l) {
-    // o in 16 bits needs P and the state to 16 bits, which leaves 2^-17 of it (one plane would do in 13% less time, but
-    // 1.4 times the error that rounding o leaves); the states are fp32 results, and so is the slope with all that goes
-    // into it: 24 bits
-    constexpr int n = std::is_same<T, float>::value ? 3 : 2;
-    if (l.states) k_chunks<T, KD, NW, 1, 1, 3, true, 0, 2><<<l.grid, 64 * NW, 0, l.stream>>>(a);
-    else if (l.slope == 1) k_chunks<T, KD, NW, n, 3, 3, false, 1, 2><<<l.grid, 64 * NW, 0, l.stream>>>(a);
-    else if (l.slope == 2) k_chunks<T, KD, NW, n, 3, 3, false, 2, 2><<<l.grid, 64 * NW, 0, l.stream>>>(a);
-    else if (l.last) k_chunks<T, KD, NW, n, n, 3, false, 0, 2><<<l.grid, 64 * NW, 0, l.stream>>>(a);
-    else k_chunks<T, KD, NW, n, n, n, false, 0, 2><<<l.grid, 64 * NW, 0, l.stream>>>(a);
+    if (l.states) k_chunks<T, KD, NW, true, 0><<<l.grid, 64 * NW, 0, l.stream>>>(a);
+    else if (l.slope == 1) k_chunks<T, KD, NW, false, 1><<<l.grid, 64 * NW, 0, l.stream>>>(a);
+    else if (l.slope == 2) k_chunks<T, KD, NW, false, 2><<<l.grid, 64 * NW, 0, l.stream>>>(a);
+    else k_chunks<T, KD, NW, false, 0><<<l.grid, 64 * NW, 0, l.stream>>>(a);
 }
 
 template <class T>
