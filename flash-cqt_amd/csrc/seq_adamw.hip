@@ -10,10 +10,22 @@
 // half the range in exponents) four exponent bits. A code's value comes out of shifts alone, no table. sqrt(v) > 0
 // never becomes code 0: a vanished spread would leave m / eps.
 //
+// A code is the nearest one, or (fcqt_adamw_drawn) one of the two neighbours, drawn so that m and v are kept on average.
+// The nearest serves a single step; over many it is wrong: a step with b2 = 0.999 takes at most 0.05% off sqrt(v), far from
+// half a code's step of 1.6 to 3.1%, so codes stay where they are. (1000 steps of unit noise leave v 1.3 of its value, drawn
+// codes 1.00; 6000 steps after gradients fell to a tenth sqrt(v) is 9 times too large, drawn 0.99, 11 to 13% off (rms).)
+// The draw is a hash of seed, step, tensor and element: the same call gives the same codes. v's chance is that of w w, not
+// of w = sqrt(v), whose square would grow by the codes' variance (2% in all). Under m's smallest code the draw takes place
+// where that code is a step of at most four learning rates (a gradient's own is up to (1 - b1) / sqrt(1 - b2), 3.2);
+// beyond, m becomes zero: an element under 2^-13 of its block's moves by its gradients alone, where the draw would be rare
+// steps of thousands of learning rates.
+//
 // Bound by memory with fp32 moments: 28 bytes an element with fp32 weights, 100 million in 512 us (5.5 TB/s; a copy 4.8).
 // With 8-bit moments and bf16 weights 10 bytes an element; 100 million take 237 us (4.2 TB/s), about 100 instructions an element
-// (exact quotients and roots) beside them, and reading them back 150 (5.4 TB/s).
+// (exact quotients and roots) beside them, drawn codes 297 (the hash: three products an element at a quarter of the rate), and
+// reading them back 150 (5.4 TB/s).
 #include <algorithm>
+#include <type_traits>
 
 #include "seq_common.hpp"
 
@@ -32,7 +44,36 @@ struct Tensors {
     uint32_t first[kMost];     // first workgroup of each tensor
     int count;
 };
-static_assert(sizeof(Tensors) + sizeof(fcqt_adamw_factors) + 32 <= 4096, "kernel arguments");
+
+// what the draws of each tensor start from
+template <bool kDraw>
+struct Keys {
+    uint64_t of[kDraw ? kMost : 1];
+};
+static_assert(sizeof(Tensors) + sizeof(fcqt_adamw_factors) + sizeof(Keys<true>) + 32 <= 4096, "kernel arguments");
+
+// A bijection of 64 bits whose every output bit depends on all input bits: products with odd numbers (of the golden ratio's
+// and the root of three's digits) carry upwards, shifts downwards.
+uint64_t mixed(uint64_t x) {
+    x ^= x >> 32;
+    x *= 0x9E3779B97F4A7C15ull;
+    x ^= x >> 29;
+    x *= 0xBB67AE8584CAA73Bull;
+    return x ^ x >> 32;
+}
+
+// Two numbers in [0, 1) for element i of a tensor, by the same means in 32 bits.
+__device__ __forceinline__ void drawn(uint64_t key, int64_t i, float& a, float& b) {
+    uint32_t x = uint32_t(i) ^ uint32_t(key) ^ uint32_t(i >> 32) * 0x85D4A0ADu;
+    x ^= x >> 16;
+    x *= 0x9E3779B1u;
+    x ^= uint32_t(key >> 32);
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    x ^= x >> 16;
+    b = float(x >> 8) * 0x1p-24f;
+    a = float(x * 0x9E3779B1u >> 8) * 0x1p-24f;
+}
 
 // the tensor that a workgroup works on
 __device__ __forceinline__ int owner(const Tensors& a, uint32_t block) {
@@ -74,9 +115,10 @@ struct Code {
 
     // inverse: 1 / scale. kNear: with a scale from 2^-70 to 2^100, where the quotient's remainder is an fp32 number (or the
     // code 0): a neighbour of the quotient, made good by its remainder times the rounded inverse, is the rounded quotient
-    // (Markstein's theorem), in five instructions instead of eleven.
-    template <bool kNear>
-    static __device__ __forceinline__ uint32_t code(float x, float scale, float inverse) {
+    // (Markstein's theorem), in five instructions instead of eleven. kDraw: the code below or the one above, by the number r
+    // in [0, 1); least: whether a first moment may become the smallest code.
+    template <bool kNear, bool kDraw>
+    static __device__ __forceinline__ uint32_t code(float x, float scale, float inverse, float r, bool least) {
 #pragma clang fp contract(off)
         const float a = fabsf(x);
         float y;
@@ -88,9 +130,23 @@ struct Code {
             y = scale > 0 ? a / scale : 0.0f;
         }
         const uint32_t bits = __float_as_uint(y);
-        const uint32_t normal = ((bits + 0x3FFFF + ((bits >> 19) & 1)) >> 19) - (bias << 4);
-        const uint32_t sub = uint32_t(int(rintf(y * float(1 << (low + 4)))));
-        uint32_t c = y < 1.0f / float(1 << low) ? sub : normal;
+        const bool small = y < 1.0f / float(1 << low);
+        const float units = y * float(1 << (low + 4));              // in the smallest codes' steps
+        uint32_t c;
+        if constexpr (kDraw) {
+            const float whole = floorf(units);
+            c = small ? uint32_t(int(whole)) : (bits >> 19) - (bias << 4);
+            const float f = small ? units - whole : float(bits & 0x7FFFF) * 0x1p-19f;       // of the way to the next code
+            if constexpr (kUnsigned) {
+                // l and l + 1 (codes in steps of their binade): (l + f)^2 lies f (2 l + f) / (2 l + 1) of the way between squares
+                const float twice = float(2 * (small ? c : 16 + (c & 15)));
+                c += r * (twice + 1) < f * (twice + f);
+            } else {
+                c += r < f && (c || least);
+            }
+        } else {
+            c = small ? uint32_t(int(rintf(units))) : ((bits + 0x3FFFF + ((bits >> 19) & 1)) >> 19) - (bias << 4);
+        }
         if (kUnsigned) return a > 0 ? min(max(c, 1u), 255u) : 0u;
         return min(c, 127u) | (x < 0 ? 128u : 0u);
     }
@@ -135,8 +191,8 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Tensors a, fcqt_adamw_factor
 }
 
 // A lane holds eight elements, half a wave one block's scale.
-template <class T>
-__global__ __launch_bounds__(kThreads) void k_adamw8(Tensors a, fcqt_adamw_factors f, const float* grad_scale) {
+template <class T, bool kDraw>
+__global__ __launch_bounds__(kThreads) void k_adamw8(Tensors a, fcqt_adamw_factors f, const float* grad_scale, Keys<kDraw> keys) {
 #pragma clang fp contract(off)
     constexpr int V = 8, kShare = kThreads * V;
     const int i = owner(a, blockIdx.x);
@@ -191,14 +247,19 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(Tensors a, fcqt_adamw_facto
     vs = __uint_as_float(max(wtop, uint32_t(__shfl_xor(int(wtop), 16)))) * float(1 / 1.9375);
     if (!some) return;
     Pack<uint8_t, V> x, y;
-    if (min(ms, vs) >= 0x1p-70f && max(ms, vs) <= 0x1p100f) {
-        const float mi = 1.0f / ms, vi = 1.0f / vs;
+    const uint64_t key = kDraw ? keys.of[i] : 0;
+    const auto codes = [&](auto near) {
+        const float mi = near ? 1.0f / ms : 0, vi = near ? 1.0f / vs : 0;
 #pragma unroll
-        for (int e = 0; e < V; ++e) x.e[e] = Code<false>::code<true>(mm[e], ms, mi), y.e[e] = Code<true>::code<true>(ww[e], vs, vi);
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) x.e[e] = Code<false>::code<false>(mm[e], ms, 0), y.e[e] = Code<true>::code<false>(ww[e], vs, 0);
-    }
+        for (int e = 0; e < V; ++e) {
+            float rm = 0, rv = 0;
+            if constexpr (kDraw) drawn(key, at + e, rm, rv);
+            x.e[e] = Code<false>::template code<near, kDraw>(mm[e], ms, mi, rm, ms * 0x1p-10f <= ww[e] * 4.0f);
+            y.e[e] = Code<true>::template code<near, kDraw>(ww[e], vs, vi, rv, true);
+        }
+    };
+    if (min(ms, vs) >= 0x1p-70f && max(ms, vs) <= 0x1p100f) codes(std::true_type{});
+    else codes(std::false_type{});
     if (wide) {
         store<T, V>(p, pp);
         *reinterpret_cast<Pack<uint8_t, V>*>(m) = x;
@@ -256,11 +317,16 @@ __global__ __launch_bounds__(kThreads) void k_adamw_read(Tensors a) {
 // goes in pieces of whole blocks. elem, moment: bytes of an element of p and g, of m and v.
 constexpr int64_t kGrid = int64_t(1) << 23;
 
+struct Place {
+    int64_t tensor, first;
+};
+
 template <class Launch>
 int in_groups(const fcqt_adamw_tensor* tensors, int64_t count, int64_t share, int elem, int moment, Launch launch) {
     int64_t at = 0, done = 0;                              // the next tensor, and how much of it has been given out
     while (at < count) {
         Tensors a;
+        Place begun[kMost];                                // which tensor each descriptor is of, and from where
         a.count = 0;
         int64_t blocks = 0;
         while (at < count && a.count < kMost && blocks < kGrid) {
@@ -271,6 +337,7 @@ int in_groups(const fcqt_adamw_tensor* tensors, int64_t count, int64_t share, in
                     return p ? static_cast<char*>(const_cast<void*>(p)) + done * bytes : nullptr;
                 };
                 const auto scale = [&](float* p) { return p ? p + done / kBlock : nullptr; };
+                begun[a.count] = {at, done};
                 a.t[a.count] = {moved(t.p, elem), moved(t.g, elem), moved(t.m, moment), moved(t.v, moment),
                                 scale(t.m_scale), scale(t.v_scale), n};
                 a.first[a.count++] = uint32_t(blocks);
@@ -280,7 +347,7 @@ int in_groups(const fcqt_adamw_tensor* tensors, int64_t count, int64_t share, in
             if (done >= t.n) ++at, done = 0;
         }
         if (!a.count) break;
-        launch(a, dim3(uint32_t(blocks)));
+        launch(a, dim3(uint32_t(blocks)), begun);
         if (int e = launched()) return e;
     }
     return FCQT_OK;
@@ -299,6 +366,19 @@ int checked(const fcqt_adamw_tensor* tensors, int64_t count, int elem, int momen
     return FCQT_OK;
 }
 
+template <class T, bool kDraw>
+void launch8(const Tensors& a, dim3 grid, const fcqt_adamw_factors& f, const float* grad_scale, const Keys<kDraw>& keys, hipStream_t stream) {
+    k_adamw8<T, kDraw><<<grid, kThreads, 0, stream>>>(a, f, grad_scale, keys);
+}
+
+template <bool kDraw>
+void launch8(const Tensors& a, dim3 grid, int32_t dtype, const fcqt_adamw_factors& f, const float* grad_scale, const Keys<kDraw>& keys,
+             hipStream_t stream) {
+    if (dtype == FCQT_F32) launch8<float>(a, grid, f, grad_scale, keys, stream);
+    else if (dtype == FCQT_BF16) launch8<bf16>(a, grid, f, grad_scale, keys, stream);
+    else launch8<f16>(a, grid, f, grad_scale, keys, stream);
+}
+
 }  // namespace
 
 extern "C" int fcqt_adamw(const fcqt_adamw_tensor* tensors, int64_t count, int32_t dtype, int32_t bits,
@@ -307,22 +387,33 @@ extern "C" int fcqt_adamw(const fcqt_adamw_tensor* tensors, int64_t count, int32
     if (int e = checked(tensors, count, size_of(dtype), bits / 8, bits == 8)) return e;
     if (!aligned(grad_scale, 4)) return FCQT_EALIGN;
     const fcqt_adamw_factors f = *factors;
-    return in_groups(tensors, count, bits == 32 ? kThreads * 4 : kThreads * 8, size_of(dtype), bits / 8, [&](const Tensors& a, dim3 grid) {
-        if (bits == 32) {
-            if (dtype == FCQT_F32) k_adamw<float><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
-            else if (dtype == FCQT_BF16) k_adamw<bf16><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
-            else k_adamw<f16><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
-        } else {
-            if (dtype == FCQT_F32) k_adamw8<float><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
-            else if (dtype == FCQT_BF16) k_adamw8<bf16><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
-            else k_adamw8<f16><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
-        }
+    return in_groups(tensors, count, bits == 32 ? kThreads * 4 : kThreads * 8, size_of(dtype), bits / 8, [&](const Tensors& a, dim3 grid, const Place*) {
+        if (bits == 8) return launch8<false>(a, grid, dtype, f, grad_scale, Keys<false>{}, stream);
+        if (dtype == FCQT_F32) k_adamw<float><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
+        else if (dtype == FCQT_BF16) k_adamw<bf16><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
+        else k_adamw<f16><<<grid, kThreads, 0, stream>>>(a, f, grad_scale);
+    });
+}
+
+extern "C" int fcqt_adamw_drawn(const fcqt_adamw_tensor* tensors, int64_t count, int32_t dtype,
+                                const fcqt_adamw_factors* factors, const float* grad_scale, uint64_t seed, int64_t step,
+                                hipStream_t stream) {
+    if (!factors || !known(dtype)) return FCQT_EARG;
+    if (int e = checked(tensors, count, size_of(dtype), 1, true)) return e;
+    if (!aligned(grad_scale, 4)) return FCQT_EALIGN;
+    const fcqt_adamw_factors f = *factors;
+    const uint64_t from = mixed(seed) + uint64_t(step);
+    return in_groups(tensors, count, kThreads * 8, size_of(dtype), 1, [&](const Tensors& a, dim3 grid, const Place* begun) {
+        Keys<true> keys;
+        for (int i = 0; i < kMost; ++i)
+            keys.of[i] = i >= a.count ? 0 : mixed(from + uint64_t(begun[i].tensor + 1) * 0x9E3779B97F4A7C15ull + uint64_t(begun[i].first) * 0xBB67AE8584CAA73Bull);
+        launch8<true>(a, grid, dtype, f, grad_scale, keys, stream);
     });
 }
 
 extern "C" int fcqt_adamw_read(const fcqt_adamw_tensor* tensors, int64_t count, hipStream_t stream) {
     if (int e = checked(tensors, count, 4, 1, true)) return e;
-    return in_groups(tensors, count, kThreads * 4, 4, 1, [&](const Tensors& a, dim3 grid) {
+    return in_groups(tensors, count, kThreads * 4, 4, 1, [&](const Tensors& a, dim3 grid, const Place*) {
         k_adamw_read<<<grid, kThreads, 0, stream>>>(a);
     });
 }

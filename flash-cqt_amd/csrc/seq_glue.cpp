@@ -34,6 +34,7 @@ struct Calls {
     decltype(&fcqt_decay_attention_bwd) attention_bwd;
     decltype(&fcqt_decay_attention_step) step;
     decltype(&fcqt_adamw) adamw;
+    decltype(&fcqt_adamw_drawn) adamw_drawn;
     decltype(&fcqt_adamw_read) read;
 } lib;
 
@@ -393,10 +394,11 @@ bool moments(const std::vector<Tensor>& m, const std::vector<Tensor>& v, const s
     return true;
 }
 
-// True when done. Tensors of one type on the current GPU; factors as _seq_native.AdamwFactors has them.
+// True when done. Tensors of one type on the current GPU; factors as _seq_native.AdamwFactors has them. seed: 8-bit codes
+// are drawn.
 bool adamw(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
            const std::vector<Tensor>& v, const std::vector<Tensor>& ms, const std::vector<Tensor>& vs, bool eight,
-           const std::vector<double>& factors, const Maybe& grad_scale) {
+           const std::vector<double>& factors, const Maybe& grad_scale, std::optional<uint64_t> seed, int64_t step) {
     const size_t n = p.size();
     if (!n || g.size() != n || m.size() != n || v.size() != n || factors.size() != 8 || !plain_call() ||
         !p[0].defined() || !p[0].is_cuda() || kind_of(p[0].scalar_type()) < 0 || (eight && (ms.size() != n || vs.size() != n)))
@@ -417,9 +419,10 @@ bool adamw(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std
     }
     const fcqt_adamw_factors f{float(factors[0]), float(factors[1]), float(factors[2]), float(factors[3]),
                                float(factors[4]), float(factors[5]), float(factors[6]), float(factors[7])};
+    const float* gs = grad_scale ? floats(*grad_scale) : nullptr;
     guarded([&] {
-        check(lib.adamw(ts.data(), int64_t(n), kind_of(type), eight ? 8 : 32, &f, grad_scale ? floats(*grad_scale) : nullptr,
-                        stream_of(p[0])),
+        check(eight && seed ? lib.adamw_drawn(ts.data(), int64_t(n), kind_of(type), &f, gs, *seed, step, stream_of(p[0]))
+                            : lib.adamw(ts.data(), int64_t(n), kind_of(type), eight ? 8 : 32, &f, gs, stream_of(p[0])),
               "adamw_step");
     });
     for (const auto* list : {&p, &m, &v, &ms, &vs})
@@ -428,12 +431,13 @@ bool adamw(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std
 }
 
 void attach(int64_t norm, int64_t norm_partial, int64_t norm_bwd, int64_t attention_workspace, int64_t attention,
-            int64_t attention_bwd, int64_t step, int64_t adamw, int64_t read) {
+            int64_t attention_bwd, int64_t step, int64_t adamw, int64_t adamw_drawn, int64_t read) {
     lib = {reinterpret_cast<decltype(lib.norm)>(norm), reinterpret_cast<decltype(lib.norm_partial)>(norm_partial),
            reinterpret_cast<decltype(lib.norm_bwd)>(norm_bwd),
            reinterpret_cast<decltype(lib.attention_workspace)>(attention_workspace),
            reinterpret_cast<decltype(lib.attention)>(attention), reinterpret_cast<decltype(lib.attention_bwd)>(attention_bwd),
            reinterpret_cast<decltype(lib.step)>(step), reinterpret_cast<decltype(lib.adamw)>(adamw),
+           reinterpret_cast<decltype(lib.adamw_drawn)>(adamw_drawn),
            reinterpret_cast<decltype(lib.read)>(read)};
 }
 

@@ -16,7 +16,7 @@ from ._native import NativeError, stream_handle  # noqa: F401
 
 LIB_PATH = _native.LIB_PATH.with_name("libflashcqt_seq.so")
 GLUE_PATH = LIB_PATH.with_name("_fcqt_seq_torch.so")
-ABI_VERSION = 1
+ABI_VERSION = 2
 MAX_DIM = 256             # FCQT_SEQ_MAX_DIM
 DECAY_MAX_DIM = 128       # FCQT_DECAY_MAX_DIM
 ROTARY_AXES = 4           # FCQT_ROTARY_AXES
@@ -28,14 +28,14 @@ EXPORTS = ("fcqt_seq_abi_version", "fcqt_seq_last_hip_error", "fcqt_head_norm_ro
            "fcqt_head_norm_rotary_partial", "fcqt_head_norm_rotary_bwd",
            "fcqt_decay_attention_workspace", "fcqt_decay_attention", "fcqt_decay_attention_bwd",
            "fcqt_decay_attention_step",
-           "fcqt_adamw", "fcqt_adamw_read")
+           "fcqt_adamw", "fcqt_adamw_drawn", "fcqt_adamw_read")
 
 #: the functions that the glue is handed, in its order
 GLUE_CALLS = ("fcqt_head_norm_rotary", "fcqt_head_norm_rotary_partial", "fcqt_head_norm_rotary_bwd",
               "fcqt_decay_attention_workspace", "fcqt_decay_attention", "fcqt_decay_attention_bwd",
-              "fcqt_decay_attention_step", "fcqt_adamw", "fcqt_adamw_read")
+              "fcqt_decay_attention_step", "fcqt_adamw", "fcqt_adamw_drawn", "fcqt_adamw_read")
 
-P, I32, I64, F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+P, I32, I64, U64, F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float
 
 
 class Heads(ctypes.Structure):
@@ -86,6 +86,7 @@ def load():
                                      ctypes.c_int),
         "fcqt_decay_attention_step": ([H, H, H, P, P, P, P, I64, I64, I32, I32, I32, F32, P], ctypes.c_int),
         "fcqt_adamw": ([ctypes.POINTER(AdamwTensor), I64, I32, I32, ctypes.POINTER(AdamwFactors), P, P], ctypes.c_int),
+        "fcqt_adamw_drawn": ([ctypes.POINTER(AdamwTensor), I64, I32, ctypes.POINTER(AdamwFactors), P, U64, I64, P], ctypes.c_int),
         "fcqt_adamw_read": ([ctypes.POINTER(AdamwTensor), I64, P], ctypes.c_int),
     }
     ver = lib.fcqt_seq_abi_version() if hasattr(lib, "fcqt_seq_abi_version") else None

@@ -8,10 +8,11 @@ A CQT layer's learnt gains and a small model's weights are dozens of small
 tensors: an elementwise launch for each of a step's operations on each of them
 takes far longer than their arithmetic. Here a launch serves up to 56 tensors.
 With state_bits=8 the moments take one byte an element and one float32 scale
-for every 256, instead of four bytes.
+for every 256, instead of four bytes; codes are drawn between a value's two
+neighbours, so that moments follow AdamW's rule over many steps.
 """
-import ctypes
 import math
+import operator
 
 import torch
 
@@ -21,6 +22,10 @@ __all__ = ["AdamW", "adamw_step", "read_moments"]
 
 
 _ORDINARY = frozenset((torch.Tensor, torch.nn.Parameter))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _blocks(n):
@@ -60,7 +65,7 @@ def _scale_lists(scales, count):
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
-               scales=None, grad_scale=None):
+               scales=None, grad_scale=None, seed=None):
     """One AdamW step (decoupled weight decay) of the tensors `params`, in place.
 
     params, grads: contiguous tensors of float32, bfloat16 or float16 on one
@@ -77,11 +82,16 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
         raise ValueError("params, grads, exp_avgs and exp_avg_sqs differ in length")
     f = _factors(step, lr, betas, eps, weight_decay)
     lists = _scale_lists(scales, count)
+    if seed is not None:
+        seed = operator.index(seed)
+        if not 0 <= seed < 1 << 64:
+            raise ValueError(f"seed is {seed}: 0 to 2^64 - 1 wanted")
+    at = 0 if seed is None else operator.index(step)
     glue = None if torch.compiler.is_compiling() else _n.load_glue()
     if glue is not None and all(
             _ORDINARY.issuperset(map(type, ts)) for ts in (params, grads, exp_avgs, exp_avg_sqs, *(lists or ()))):
         ms, vs = lists or ((), ())
-        if glue.adamw(params, grads, exp_avgs, exp_avg_sqs, ms, vs, lists is not None, f, grad_scale):
+        if glue.adamw(params, grads, exp_avgs, exp_avg_sqs, ms, vs, lists is not None, f, grad_scale, seed, at):
             return
     bits = 32 if lists is None else 8
     state = (torch.float32,) if bits == 32 else (torch.uint8,)
@@ -96,13 +106,16 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
                            None if lists is None else _scale(f"scales[0][{i}]", lists[0][i], p),
                            None if lists is None else _scale(f"scales[1][{i}]", lists[1][i], p), p.numel())
         groups.setdefault((p.dtype, p.device), []).append(d)
-    for (dtype, device), ds in groups.items():
+    for i, ((dtype, device), ds) in enumerate(groups.items()):
         if grad_scale is not None and grad_scale.device != device:
             raise ValueError(f"grad_scale is on {grad_scale.device}, a tensor on {device}")
-        _n.check(_n.load().fcqt_adamw((_n.AdamwTensor * len(ds))(*ds), len(ds), _n.DTYPES[dtype], bits,
-                                      _n.AdamwFactors(*f),
-                                      None if grad_scale is None else grad_scale.data_ptr(),
-                                      _n.stream_handle(device.index)), "adamw_step")
+        ts, gs, stream = (_n.AdamwTensor * len(ds))(*ds), _ptr(grad_scale), _n.stream_handle(device.index)
+        if bits == 8 and seed is not None:
+            status = _n.load().fcqt_adamw_drawn(ts, len(ds), _n.DTYPES[dtype], _n.AdamwFactors(*f), gs,
+                                                (seed + (i << 48)) % (1 << 64), at, stream)
+        else:
+            status = _n.load().fcqt_adamw(ts, len(ds), _n.DTYPES[dtype], bits, _n.AdamwFactors(*f), gs, stream)
+        _n.check(status, "adamw_step")
     torch.autograd.graph.increment_version([*params, *exp_avgs, *exp_avg_sqs, *(x for xs in lists or () for x in xs)])
 
 
@@ -139,14 +152,19 @@ def read_moments(exp_avgs, exp_avg_sqs, scales, *, out=None):
 class AdamW(torch.optim.Optimizer):
     """torch.optim's interface over adamw_step: parameter groups, schedulers,
     state_dict. state_bits: 32, or 8 for one byte a moment (decided when a
-    parameter first steps; tensors under min_8bit elements keep 32 bits)."""
+    parameter first steps; tensors under min_8bit elements keep 32 bits).
+    seed: of the draws that 8-bit moments are rounded by (adamw_step); runs of
+    one seed and the same gradients are the same."""
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit=4096):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit=4096,
+                 seed=0):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits is {state_bits}: 8 or 32 wanted")
+        if not 0 <= operator.index(seed) < 1 << 32:
+            raise ValueError(f"seed is {seed}: 0 to 2^32 - 1 wanted")
         _factors(1, lr, betas, eps, weight_decay)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      min_8bit=min_8bit))
+                                      min_8bit=min_8bit, seed=seed))
 
     def _state(self, p, group):
         s = self.state[p]
@@ -165,6 +183,9 @@ class AdamW(torch.optim.Optimizer):
         """As torch.optim's, which casts a state to its parameter's type: codes
         and scales keep theirs."""
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            for name, x in self.defaults.items():
+                group.setdefault(name, x)
         index = {i: p for g, h in zip(state_dict["param_groups"], self.param_groups)
                  for i, p in zip(g["params"], h["params"])}
         for i, s in state_dict["state"].items():
@@ -182,7 +203,7 @@ class AdamW(torch.optim.Optimizer):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step under stream capture would replay one step's factors; capture adamw_step "
                                "only where that is meant")
-        for group in self.param_groups:
+        for i, group in enumerate(self.param_groups):
             # tensors of one count of steps and one kind of moments go together
             sets = {}
             for p in group["params"]:
@@ -197,5 +218,6 @@ class AdamW(torch.optim.Optimizer):
                 scales = tuple([s[n] for _, _, s in ps] for n in ("exp_avg_scale", "exp_avg_sq_scale")) if eight else None
                 adamw_step([p for p, _, _ in ps], [g for _, g, _ in ps], [s["exp_avg"] for _, _, s in ps],
                            [s["exp_avg_sq"] for _, _, s in ps], step=step, lr=group["lr"], betas=group["betas"],
-                           eps=group["eps"], weight_decay=group["weight_decay"], scales=scales, grad_scale=grad_scale)
+                           eps=group["eps"], weight_decay=group["weight_decay"], scales=scales, grad_scale=grad_scale,
+                           seed=group["seed"] + (i << 32))
         return loss

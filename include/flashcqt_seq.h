@@ -5,7 +5,8 @@
  *   fcqt_decay_attention          linear attention with a decay for each head, over whole sequences; run forwards
  *                                 or backwards in time it also gives its own gradients
  *   fcqt_decay_attention_step     the same for one token of every running sequence, states in a pool
- *   fcqt_adamw, fcqt_adamw_read   one AdamW step over many tensors, moments in 32 or in 8 bits
+ *   fcqt_adamw, fcqt_adamw_drawn, fcqt_adamw_read
+ *                                 one AdamW step over many tensors, moments in 32 or in 8 bits
  *
  * Conventions, as in flashcqt.h: every buffer is device memory of the caller's, nothing is allocated; all work is
  * enqueued on `stream`, which may be under hipGraph capture; argument errors are found before any HIP call and
@@ -23,7 +24,7 @@
 extern "C" {
 #endif
 
-#define FCQT_SEQ_ABI_VERSION 1
+#define FCQT_SEQ_ABI_VERSION 2
 
 /* element types */
 #define FCQT_F32 0
@@ -128,9 +129,15 @@ typedef struct fcqt_adamw_factors {
 } fcqt_adamw_factors;
 
 /* `tensors` is host memory, read before the call returns. dtype: of p and g. grad_scale: NULL, or a device scalar
- * that every gradient is multiplied by first. Tensors of no elements are passed over. */
+ * that every gradient is multiplied by first. Tensors of no elements are passed over. With bits = 8 every moment gets
+ * its nearest code, which is not for many steps: a moment that a step changes by less than half a code's step stays. */
 int fcqt_adamw(const fcqt_adamw_tensor* tensors, int64_t count, int32_t dtype, int32_t bits,
                const fcqt_adamw_factors* factors, const float* grad_scale, hipStream_t stream);
+
+/* With 8-bit moments, over many steps: each code is one of its value's two neighbours, drawn by a hash of seed, step,
+ * the tensor's place in the list and the element, so that m and v are kept on average. `step` is another one at each call. */
+int fcqt_adamw_drawn(const fcqt_adamw_tensor* tensors, int64_t count, int32_t dtype, const fcqt_adamw_factors* factors,
+                     const float* grad_scale, uint64_t seed, int64_t step, hipStream_t stream);
 
 /* The values that 8-bit moments stand for: p and g of each tensor name fp32 [n] buffers for m and v. */
 int fcqt_adamw_read(const fcqt_adamw_tensor* tensors, int64_t count, hipStream_t stream);
