@@ -128,10 +128,13 @@ variable_list once(variable_list g) {
 
 Tensor contiguous_last(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
+// t as a node saves it, no input of its graph
+Tensor saved_form(const Tensor& t) { return !t.defined() ? t : t.is_inference() ? t.clone() : t.detach(); }
+
 // ------------------------------------------------- head norm and rotary positions
 
 struct Rotary : torch::CustomClassHolder {
-    Tensor positions, freq;
+    Tensor positions, freq;         // until the node has saved them
     fcqt_rotary rot{};
     double eps;
     bool norm;
@@ -153,7 +156,9 @@ struct NormRotary : torch::autograd::Function<NormRotary> {
                                  const Maybe& wk_, const Turn& r) {
         const Tensor wq = wq_.value_or(Tensor()), wk = wk_.value_or(Tensor());
         ctx->saved_data["turn"] = c10::IValue::make_capsule(r);
-        ctx->save_for_backward({q, k, wq, wk});
+        // (positions and frequencies are saved too: a change of them in place before the backward pass is seen)
+        ctx->save_for_backward({q, k, wq, wk, saved_form(r->positions), saved_form(r->freq)});
+        r->positions = r->freq = Tensor();
         return norm_rotary_out(q, k, wq, wk, *r);
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& g) {
@@ -163,6 +168,8 @@ struct NormRotary : torch::autograd::Function<NormRotary> {
             at::AutoGradMode off(false);
             const Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3];
             const Turn r = c10::static_intrusive_pointer_cast<Rotary>(ctx->saved_data["turn"].toCapsule());
+            fcqt_rotary rot = r->rot;
+            rot.positions = floats(saved[4]), rot.freq = floats(saved[5]);
             const Tensor gq = contiguous_last(g[0]), gk = contiguous_last(g[1]);
             const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
             const int64_t B = q.size(0), T = q.size(1);
@@ -176,7 +183,7 @@ struct NormRotary : torch::autograd::Function<NormRotary> {
             }
             if (some) {
                 const fcqt_heads hq = heads(q), hk = heads(k), hgq = heads(gq), hgk = heads(gk);
-                check(lib.norm_bwd(&hq, &hk, &hgq, &hgk, &r->rot, floats(wq), floats(wk), dq.data_ptr(), dk.data_ptr(),
+                check(lib.norm_bwd(&hq, &hk, &hgq, &hgk, &rot, floats(wq), floats(wk), dq.data_ptr(), dk.data_ptr(),
                                    floats(dw), floats(partial), B, T, D, kind, r->norm, float(r->eps), stream_of(q)),
                       "head_norm_rotary backward");
             }

@@ -117,14 +117,19 @@ def head_norm_rotary(q, k, positions=None, freq=None, sections=(), wq=None, wk=N
         positions = positions.detach().float().contiguous()
         _need(freq is not None, "positions without freq")
         freq = _floats("freq", freq.detach(), (pairs,), q.device)
-    how = (positions, freq, sections, float(eps), bool(interleaved), bool(norm))
+    how = (sections, float(eps), bool(interleaved), bool(norm))
     if _wants_grad(q, k, wq, wk):
-        return _HeadNormRotary.apply(q, k, wq, wk, how)
-    return _head_norm_rotary(q, k, wq, wk, how)
+        return _HeadNormRotary.apply(q, k, wq, wk, _saved(positions), _saved(freq), how)
+    return _head_norm_rotary(q, k, wq, wk, positions, freq, how)
 
 
-def _rotary(how):
-    positions, freq, sections, _, interleaved, _ = how
+def _saved(t):
+    """t as it can be saved for the backward pass."""
+    return t.clone() if t is not None and t.is_inference() else t
+
+
+def _rotary(positions, freq, how):
+    sections, _, interleaved, _ = how
     r = _n.Rotary()
     if positions is not None and sum(sections):
         r.positions, r.freq = positions.data_ptr(), freq.data_ptr()
@@ -141,28 +146,28 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _head_norm_rotary(q, k, wq, wk, how):
+def _head_norm_rotary(q, k, wq, wk, positions, freq, how):
     q, k = _in_place(q), _in_place(k)
     B, T, _, D = q.shape
     oq, ok = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
     if B * T:
-        _n.check(_n.load().fcqt_head_norm_rotary(_n.heads(q), _n.heads(k), _rotary(how), _ptr(wq), _ptr(wk),
-                                                 oq.data_ptr(), ok.data_ptr(), B, T, D, _n.DTYPES[q.dtype], how[5],
-                                                 how[3], _n.stream_handle(q.device.index)), "head_norm_rotary")
+        _n.check(_n.load().fcqt_head_norm_rotary(_n.heads(q), _n.heads(k), _rotary(positions, freq, how), _ptr(wq),
+                                                 _ptr(wk), oq.data_ptr(), ok.data_ptr(), B, T, D, _n.DTYPES[q.dtype],
+                                                 how[3], how[1], _n.stream_handle(q.device.index)), "head_norm_rotary")
     return oq, ok
 
 
 class _HeadNormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, how):
+    def forward(ctx, q, k, wq, wk, positions, freq, how):
         ctx.how = how
-        ctx.save_for_backward(q, k, wq, wk)
-        return _head_norm_rotary(q, k, wq, wk, how)
+        ctx.save_for_backward(q, k, wq, wk, positions, freq)
+        return _head_norm_rotary(q, k, wq, wk, positions, freq, how)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk = ctx.saved_tensors
+        q, k, wq, wk, positions, freq = ctx.saved_tensors
         how = ctx.how
         q, k, gq, gk = (_in_place(t) for t in (q, k, gq, gk))
         B, T, _, D = q.shape
@@ -176,11 +181,11 @@ class _HeadNormRotary(torch.autograd.Function):
             kind = _n.DTYPES[q.dtype]
             partial = dw if dw is None else torch.empty(
                 lib.fcqt_head_norm_rotary_partial(B, T, q.shape[2] + k.shape[2], D, kind), dtype=torch.float32, device=q.device)
-            _n.check(lib.fcqt_head_norm_rotary_bwd(_n.heads(q), _n.heads(k), _n.heads(gq), _n.heads(gk), _rotary(how),
-                                                   _ptr(wq), _ptr(wk), dq.data_ptr(), dk.data_ptr(), _ptr(dw),
-                                                   _ptr(partial), B, T, D, kind, how[5], how[3],
+            _n.check(lib.fcqt_head_norm_rotary_bwd(_n.heads(q), _n.heads(k), _n.heads(gq), _n.heads(gk),
+                                                   _rotary(positions, freq, how), _ptr(wq), _ptr(wk), dq.data_ptr(),
+                                                   dk.data_ptr(), _ptr(dw), _ptr(partial), B, T, D, kind, how[3], how[1],
                                                    _n.stream_handle(q.device.index)), "head_norm_rotary backward")
-        return dq, dk, None if wq is None else dw[0], None if wk is None else dw[1], None
+        return dq, dk, None if wq is None else dw[0], None if wk is None else dw[1], None, None, None
 
 
 # ------------------------------------------------------- attention with a decay

@@ -1,0 +1,62 @@
+"""How the sequence operators sit in autograd: what is changed between forward
+and backward is seen, by the host glue and by the Python paths."""
+import pytest
+import torch
+
+import seq_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["glue", "python"])
+def path(request, monkeypatch):
+    from flash_cqt import _seq_native
+    if request.param == "python":
+        monkeypatch.setattr(_seq_native, "load_glue", lambda: None)
+    return request.param
+
+
+@pytest.mark.parametrize("which", ["positions", "freq"])
+def test_positions_changed_before_the_backward_pass(path, which):
+    """They are needed again, so a change in place raises; one after it, or
+    without gradients, does not."""
+    from flash_cqt import sequence
+    q = torch.randn(2, 5, 2, 16, device="cuda", requires_grad=True)
+    pos, freq = torch.rand(5, 1, device="cuda") * 9, sequence.rotary_frequencies((8,))
+    changed = pos if which == "positions" else freq
+    y, _ = sequence.head_norm_rotary(q, q, pos, freq, (8,))
+    changed.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    y, _ = sequence.head_norm_rotary(q, q, pos, freq, (8,))
+    y.square().sum().backward()
+    changed.add_(1)
+    with torch.no_grad():
+        sequence.head_norm_rotary(q, q, pos, freq, (8,))
+        changed.add_(1)
+
+
+def test_positions_of_other_kinds(path):
+    """Whole numbers, a view, values made in inference mode, values with a
+    gradient of their own: the same gradients, none of them for positions."""
+    from flash_cqt import sequence
+    x = torch.randn(2, 5, 2, 16, device="cuda")
+    freq = sequence.rotary_frequencies((8,))
+    whole = torch.tensor([[3], [1], [4], [1], [5]], device="cuda")
+    with torch.inference_mode():
+        inferred = whole.float()
+    leaf = whole.float().requires_grad_(True)
+    found = []
+    for pos in (whole, whole.float(), torch.stack([whole.float()] * 3)[1], inferred, leaf):
+        q = x.clone().requires_grad_(True)
+        y, z = sequence.head_norm_rotary(q, q, pos, freq, (8,))
+        ((y * x).sum() + z.sum()).backward()
+        found.append(q.grad)
+        if pos is whole:
+            whole += 0                                                       # converted: a copy of its own was kept
+    assert leaf.grad is None and all(torch.equal(found[0], g) for g in found[1:])
+    wide = x.cpu().double().requires_grad_(True)
+    angle = ref.angles(whole.cpu().expand(2, 5, 1), freq.cpu(), (8,))
+    y = ref.head_norm_rotary(wide, None, angle, 1e-6, False)
+    ((y * wide.detach()).sum() + y.sum()).backward()
+    ref.close(found[0], wide.grad, slack=2)
