@@ -10,6 +10,7 @@ import ctypes
 import importlib.util
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._native import NativeError, stream_handle  # noqa: F401
@@ -138,6 +139,12 @@ def check(status, what):
     if status != 0:
         hip = load().fcqt_seq_last_hip_error().decode() if status == 3 else ""
         raise NativeError(f"{what}: {STATUS.get(status, status)}" + (f" [{hip}]" if hip else ""))
+
+
+def no_tangents(*tensors):
+    """The kernels have no forward-mode derivatives: without this the outputs would have none either."""
+    if any(torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the sequence operators have no forward-mode derivatives")
 
 
 def heads(t):

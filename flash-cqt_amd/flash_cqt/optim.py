@@ -93,6 +93,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
         ms, vs = lists or ((), ())
         if glue.adamw(params, grads, exp_avgs, exp_avg_sqs, ms, vs, lists is not None, f, grad_scale, seed, at):
             return
+    _n.no_tangents(*params, *grads, *exp_avgs, *exp_avg_sqs, grad_scale)
     bits = 32 if lists is None else 8
     state = (torch.float32,) if bits == 32 else (torch.uint8,)
     if grad_scale is not None and not (torch.is_tensor(grad_scale) and grad_scale.is_cuda and grad_scale.numel() == 1

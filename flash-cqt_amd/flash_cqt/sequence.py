@@ -95,6 +95,7 @@ def head_norm_rotary(q, k, positions=None, freq=None, sections=(), wq=None, wk=N
         out = glue.norm_rotary(q, k, positions, freq, sections, wq, wk, eps, interleaved, norm)
         if out is not None:
             return out
+    _n.no_tangents(q, k, positions, freq, wq, wk)
     _heads_of("q", q, 4)
     _heads_of("k", k, 4, q.dtype, q.device)
     B, T, _, D = q.shape
@@ -220,6 +221,7 @@ def decay_attention(q, k, v, log_decay, *, scale=None, state=None, lengths=None)
         out = glue.attention(q, k, v, log_decay, state, lengths, scale)
         if out is not None:
             return out
+    _n.no_tangents(q, k, v, log_decay, state)
     decay = _attention_inputs(q, k, v, log_decay, 4, 2)
     B, T, Hq, Dk = q.shape
     Hk, Dv = v.shape[2:]
@@ -315,6 +317,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, slots=None, scale=None):
         out = glue.step(q, k, v, log_decay, state, slots, scale)
         if out is not None:
             return out
+    _n.no_tangents(q, k, v, log_decay, state)
     decay = _attention_inputs(q, k, v, log_decay, 3, 1)
     _need(not _wants_grad(q, k, v, log_decay, state), "decay_attention_step records no gradients: use decay_attention")
     B, Hq, Dk = q.shape

@@ -60,3 +60,38 @@ def test_positions_of_other_kinds(path):
     y = ref.head_norm_rotary(wide, None, angle, 1e-6, False)
     ((y * wide.detach()).sum() + y.sum()).backward()
     ref.close(found[0], wide.grad, slack=2)
+
+
+def test_forward_mode_is_refused(path):
+    """Tangents of any input raise, by dual tensors and by torch.func; so do its other transforms."""
+    import torch.autograd.forward_ad as fwd
+    from flash_cqt import sequence
+    x = torch.randn(2, 3, 2, 16, device="cuda")
+    w, pos, freq = torch.ones(16, device="cuda"), torch.rand(3, 1, device="cuda"), sequence.rotary_frequencies((8,))
+    g, S = -torch.rand(2, device="cuda"), torch.randn(2, 2, 16, 16, device="cuda")
+    calls = [(lambda q, k, w, p, f: sequence.head_norm_rotary(q, k, p, f, (8,), w)[0], (x, x, w, pos, freq)),
+             (lambda q, k, v, g, S: sequence.decay_attention(q, k, v, g, state=S)[0], (x, x, x, g, S)),
+             (lambda q, k, v, g, S: sequence.decay_attention_step(q, k, v, g, S), (x[:, 0], x[:, 0], x[:, 0], g, S.clone()))]
+    for call, args in calls:
+        call(*args)
+        for i in range(len(args)):
+            for leaf in (False, True):
+                with fwd.dual_level():
+                    t = args[i].clone().requires_grad_(leaf and call is not calls[2][0])
+                    with pytest.raises(NotImplementedError):
+                        call(*args[:i], fwd.make_dual(t, torch.ones_like(t)), *args[i + 1:])
+            with pytest.raises(RuntimeError):                                # NotImplementedError among them
+                torch.func.jvp(lambda t: call(*args[:i], t, *args[i + 1:]), (args[i],), (torch.ones_like(args[i]),))
+        with fwd.dual_level():
+            call(*args)
+        for transform in (torch.func.vmap, lambda f: torch.func.grad(lambda t: f(t).sum())):
+            with pytest.raises((RuntimeError, ValueError)):
+                transform(lambda t: call(t, *args[1:]))(args[0][None].expand(3, *args[0].shape) if transform is torch.func.vmap else args[0])
+    from flash_cqt import optim
+    p, m = torch.ones(4, device="cuda"), torch.zeros(4, device="cuda")
+    with fwd.dual_level():
+        for i in range(2):
+            t = [fwd.make_dual(p.clone(), p.clone()) if i == j else p.clone() for j in range(2)]
+            with pytest.raises(NotImplementedError):
+                optim.adamw_step([t[0]], [t[1]], [m], [m.clone()], step=1, lr=0.1)
+    assert not m.any()
