@@ -243,11 +243,19 @@ py::object norm_rotary(const Tensor& q, const Tensor& k, const Maybe& positions,
 
 // ------------------------------------------------------- attention with a decay
 
+bool placed(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
 // whether the kernels over whole sequences can read it as it lies (16 bytes at a time, 32-bit offsets inside a chunk)
 bool wide(const Tensor& t) {
     const int64_t e = t.element_size(), b = t.stride(0), n = t.stride(1), h = t.stride(2);
-    return t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (b | n | h) * e % 16 == 0 &&
+    return t.stride(3) == 1 && placed(t) && (b | n | h) * e % 16 == 0 &&
            n >= 0 && n <= (int64_t(1) << 31) / (64 * e) - FCQT_DECAY_MAX_DIM;
+}
+
+// contiguous, at a multiple of 16 bytes
+Tensor made_placed(const Tensor& t) {
+    const Tensor c = t.contiguous();
+    return placed(c) ? c : c.clone();
 }
 
 Tensor made_wide(const Tensor& t) { return wide(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
@@ -298,7 +306,7 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
             const int64_t B = q.size(0), T = q.size(1);
             const Tensor go = grads[0].defined() ? made_wide(grads[0])
                                                  : at::zeros({B, T, q.size(2), v.size(3)}, q.options());
-            const Tensor glast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+            const Tensor glast = grads[1].defined() ? made_placed(grads[1]) : Tensor();
             const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
             const Tensor dv = at::empty(v.sizes(), v.options());
             const Tensor dg = ctx->needs_input_grad(3) ? at::empty(g.sizes(), g.options()) : Tensor();
@@ -335,6 +343,7 @@ py::object attention(const Tensor& q, const Tensor& k, const Tensor& v, const Te
     if (!attention_fits(q, k, v, g, 4, FCQT_DECAY_MAX_DIM) || q.size(0) > 65535 || !wide(q) || !wide(k) || !wide(v))
         return py::none();
     if (!plain_or_none(state, at::kFloat) || !plain_or_none(lengths, at::kInt)) return py::none();
+    if (state.defined() && !placed(state)) return py::none();        // (the Python path copies it)
     if (state.defined() && state.sizes() != at::IntArrayRef({q.size(0), k.size(2), q.size(3), v.size(3)})) return py::none();
     if (lengths.defined() && (lengths.dim() != 1 || lengths.size(0) != q.size(0))) return py::none();
     const double scale = scale_.value_or(std::pow(double(q.size(3)), -0.5));

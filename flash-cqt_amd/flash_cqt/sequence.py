@@ -64,6 +64,11 @@ def _floats(name, t, shape, device):
     return t.contiguous()
 
 
+def _aligned(t):
+    """t, contiguous, or a copy at a multiple of 16 bytes."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
 # ------------------------------------------------- head norm and rotary positions
 
 def rotary_frequencies(sections, base=10000.0, device="cuda"):
@@ -228,7 +233,7 @@ def decay_attention(q, k, v, log_decay, *, scale=None, state=None, lengths=None)
     _need(max(Dk, Dv) <= _n.DECAY_MAX_DIM, f"heads of {Dk} and {Dv}: at most {_n.DECAY_MAX_DIM}")
     _need(B <= 65535, f"{B} rows: at most 65535 in one call")
     if state is not None:
-        state = _floats("state", state, (B, Hk, Dk, Dv), q.device)
+        state = _aligned(_floats("state", state, (B, Hk, Dk, Dv), q.device))
     if lengths is not None:
         _need(torch.is_tensor(lengths) and lengths.dtype == torch.int32 and tuple(lengths.shape) == (B,)
               and lengths.device == q.device, f"lengths must be an int32 tensor [{B}] beside q")
@@ -288,7 +293,7 @@ class _DecayAttention(torch.autograd.Function):
         B, T, Hq, Dk = q.shape
         Hk, Dv = v.shape[2:]
         go = torch.zeros(B, T, Hq, Dv, dtype=q.dtype, device=q.device) if go is None else _wide(go)
-        glast = None if glast is None else glast.contiguous()
+        glast = None if glast is None else _aligned(glast.contiguous())
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         dg = torch.empty_like(decay) if ctx.needs_input_grad[3] else None
         ds = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None

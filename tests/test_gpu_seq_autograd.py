@@ -95,3 +95,33 @@ def test_forward_mode_is_refused(path):
             with pytest.raises(NotImplementedError):
                 optim.adamw_step([t[0]], [t[1]], [m], [m.clone()], step=1, lr=0.1)
     assert not m.any()
+
+
+def at_odd_place(t, by=3):
+    """The same values in a contiguous view that starts at no multiple of 16 bytes."""
+    flat = torch.cat([t.new_zeros(by), t.flatten()])
+    return flat[by:].view(t.shape)
+
+
+@pytest.mark.parametrize("T", [5, 700])                                      # one segment, and several
+def test_states_at_any_place(path, T):
+    """A first state in a view at an odd place, and the gradient of a last state
+    that was joined behind three numbers, which autograd hands over as such a
+    view: the bits of those at other places."""
+    from flash_cqt import sequence
+    gen = torch.Generator("cuda").manual_seed(3)
+    q, k, v = (torch.randn(2, T, 2, 16, device="cuda", generator=gen) for _ in range(3))
+    g, S = -torch.rand(2, device="cuda", generator=gen), torch.randn(2, 2, 16, 16, device="cuda", generator=gen)
+    more, weight = torch.zeros(3, device="cuda"), torch.randn(2 * 2 * 16 * 16, device="cuda", generator=gen)
+    found = []
+    for odd in (False, True):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v, g, S)]
+        first = at_odd_place(leaves[4]) if odd else leaves[4]
+        assert (first.data_ptr() % 16 != 0) == odd
+        o, last = sequence.decay_attention(*leaves[:4], state=first)
+        joined = torch.cat([more, last.flatten()])[3:] if odd else last.flatten()
+        found.append([o, last, *torch.autograd.grad((joined * weight).sum() + o.sum(), leaves)])
+    assert all(torch.equal(a, b) for a, b in zip(*found))
+    with torch.no_grad():
+        _, last = sequence.decay_attention(q, k, v, g, state=at_odd_place(S, 1))
+    assert torch.equal(last, found[0][1])
