@@ -128,6 +128,38 @@ variable_list once(variable_list g) {
 
 Tensor contiguous_last(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
+// What a node saves. Saved-tensor hooks may give it back with other strides, but nothing else may have changed.
+struct Kept : torch::CustomClassHolder {
+    struct One {
+        at::DimVector sizes;
+        at::ScalarType type;
+        at::Device device;
+    };
+    std::vector<std::optional<One>> all;
+};
+
+void keep(AutogradContext* ctx, const variable_list& list) {
+    const auto k = c10::make_intrusive<Kept>();
+    for (const Tensor& t : list)
+        k->all.push_back(t.defined() ? std::optional<Kept::One>({at::DimVector(t.sizes()), t.scalar_type(), t.device()}) : std::nullopt);
+    ctx->saved_data["kept"] = c10::IValue::make_capsule(k);
+    ctx->save_for_backward(list);
+}
+
+variable_list kept(AutogradContext* ctx) {
+    const auto k = c10::static_intrusive_pointer_cast<Kept>(ctx->saved_data["kept"].toCapsule());
+    variable_list list = ctx->get_saved_variables();
+    for (size_t i = 0; i < list.size(); ++i) {
+        const auto& one = k->all[i];
+        TORCH_CHECK(!one || (list[i].defined() && list[i].sizes() == at::IntArrayRef(one->sizes) && list[i].scalar_type() == one->type &&
+                             list[i].device() == one->device),
+                    "a saved tensor came back with another shape, type or device");
+    }
+    return list;
+}
+
+Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
 // t as a node saves it, no input of its graph
 Tensor saved_form(const Tensor& t) { return !t.defined() ? t : t.is_inference() ? t.clone() : t.detach(); }
 
@@ -157,19 +189,20 @@ struct NormRotary : torch::autograd::Function<NormRotary> {
         const Tensor wq = wq_.value_or(Tensor()), wk = wk_.value_or(Tensor());
         ctx->saved_data["turn"] = c10::IValue::make_capsule(r);
         // (positions and frequencies are saved too: a change of them in place before the backward pass is seen)
-        ctx->save_for_backward({q, k, wq, wk, saved_form(r->positions), saved_form(r->freq)});
+        keep(ctx, {q, k, wq, wk, saved_form(r->positions), saved_form(r->freq)});
         r->positions = r->freq = Tensor();
         return norm_rotary_out(q, k, wq, wk, *r);
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-        const auto saved = ctx->get_saved_variables();
+        const auto saved = kept(ctx);
         variable_list out;
         {
             at::AutoGradMode off(false);
-            const Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3];
+            const Tensor q = contiguous_last(saved[0]), k = contiguous_last(saved[1]), wq = contiguous(saved[2]);
+            const Tensor wk = contiguous(saved[3]), positions = contiguous(saved[4]), freq = contiguous(saved[5]);
             const Turn r = c10::static_intrusive_pointer_cast<Rotary>(ctx->saved_data["turn"].toCapsule());
             fcqt_rotary rot = r->rot;
-            rot.positions = floats(saved[4]), rot.freq = floats(saved[5]);
+            rot.positions = floats(positions), rot.freq = floats(freq);
             const Tensor gq = contiguous_last(g[0]), gk = contiguous_last(g[1]);
             const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
             const int64_t B = q.size(0), T = q.size(1);
@@ -254,8 +287,8 @@ bool wide(const Tensor& t) {
 
 // contiguous, at a multiple of 16 bytes
 Tensor made_placed(const Tensor& t) {
-    const Tensor c = t.contiguous();
-    return placed(c) ? c : c.clone();
+    const Tensor c = contiguous(t);
+    return !c.defined() || placed(c) ? c : c.clone();
 }
 
 Tensor made_wide(const Tensor& t) { return wide(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
@@ -291,22 +324,22 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
         ctx->set_materialize_grads(false);
         ctx->saved_data["scale"] = scale;
         variable_list y = attention_out(q, k, v, g, state, lengths, scale);
-        ctx->save_for_backward({q, k, v, g, state, lengths, y[2]});     // the workspace: states that segments start from
+        keep(ctx, {q, k, v, g, state, lengths, y[2]});                  // the workspace: states that segments start from
         y.pop_back();
         return y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         variable_list out(7);
         if (!grads[0].defined() && !grads[1].defined()) return out;
-        const auto saved = ctx->get_saved_variables();
+        const auto saved = kept(ctx);
         {
             at::AutoGradMode off(false);
-            const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &g = saved[3], &state = saved[4];
-            const Tensor &lengths = saved[5], &starts = saved[6];
+            const Tensor q = made_wide(saved[0]), k = made_wide(saved[1]), v = made_wide(saved[2]), g = contiguous(saved[3]);
+            const Tensor state = made_placed(saved[4]), lengths = contiguous(saved[5]), starts = made_placed(saved[6]);
             const int64_t B = q.size(0), T = q.size(1);
             const Tensor go = grads[0].defined() ? made_wide(grads[0])
                                                  : at::zeros({B, T, q.size(2), v.size(3)}, q.options());
-            const Tensor glast = grads[1].defined() ? made_placed(grads[1]) : Tensor();
+            const Tensor glast = made_placed(grads[1]);
             const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
             const Tensor dv = at::empty(v.sizes(), v.options());
             const Tensor dg = ctx->needs_input_grad(3) ? at::empty(g.sizes(), g.options()) : Tensor();

@@ -69,6 +69,24 @@ def _aligned(t):
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _keep(ctx, *tensors):
+    """Save tensors for the backward pass, and what they are."""
+    ctx.kept = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+    ctx.save_for_backward(*tensors)
+
+
+def _kept(ctx):
+    """The saved tensors, as saved-tensor hooks may have changed them: of any strides, but nothing else."""
+    tensors = ctx.saved_tensors
+    if any(k is not None and k != (t.shape, t.dtype, t.device) for k, t in zip(ctx.kept, tensors)):
+        raise RuntimeError("a saved tensor came back with another shape, type or device")
+    return tensors
+
+
+def _contiguous(*tensors):
+    return [None if t is None else t.contiguous() for t in tensors]
+
+
 # ------------------------------------------------- head norm and rotary positions
 
 def rotary_frequencies(sections, base=10000.0, device="cuda"):
@@ -167,13 +185,14 @@ class _HeadNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, positions, freq, how):
         ctx.how = how
-        ctx.save_for_backward(q, k, wq, wk, positions, freq)
+        _keep(ctx, q, k, wq, wk, positions, freq)
         return _head_norm_rotary(q, k, wq, wk, positions, freq, how)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk, positions, freq = ctx.saved_tensors
+        q, k, wq, wk, positions, freq = _kept(ctx)
+        wq, wk, positions, freq = _contiguous(wq, wk, positions, freq)
         how = ctx.how
         q, k, gq, gk = (_in_place(t) for t in (q, k, gq, gk))
         B, T, _, D = q.shape
@@ -281,15 +300,17 @@ class _DecayAttention(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.scale = scale
         o, last, work = _decay_attention(q, k, v, decay, state, lengths, scale)
-        ctx.save_for_backward(q, k, v, decay, state, lengths, work)     # work: the states that segments start from
+        _keep(ctx, q, k, v, decay, state, lengths, work)                # work: the states that segments start from
         return o, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go, glast):
-        q, k, v, decay, state, lengths, starts = ctx.saved_tensors
         if go is None and glast is None:
             return (None,) * 7
+        q, k, v, decay, state, lengths, starts = _kept(ctx)
+        decay, state, lengths, starts = _contiguous(decay, state, lengths, starts)
+        state, starts = _aligned(state), _aligned(starts)
         B, T, Hq, Dk = q.shape
         Hk, Dv = v.shape[2:]
         go = torch.zeros(B, T, Hq, Dv, dtype=q.dtype, device=q.device) if go is None else _wide(go)

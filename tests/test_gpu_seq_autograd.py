@@ -125,3 +125,32 @@ def test_states_at_any_place(path, T):
     with torch.no_grad():
         _, last = sequence.decay_attention(q, k, v, g, state=at_odd_place(S, 1))
     assert torch.equal(last, found[0][1])
+
+
+def spread(t):
+    """The same values, elements of the last dimension (of a vector, its own) two places apart."""
+    return t.new_empty(*t.shape, 2)[..., 0].copy_(t)
+
+
+def test_saved_tensors_with_other_strides(path):
+    """Hooks may give saved tensors back laid out differently: the same gradients.
+    Another type, or another shape, raises."""
+    from flash_cqt import sequence
+    gen = torch.Generator("cuda").manual_seed(6)
+    q, k, v = (torch.randn(2, 700, h, 16, device="cuda", generator=gen) for h in (4, 2, 2))
+    w, g, S = (torch.rand(*s, device="cuda", generator=gen) for s in ((16,), (2,), (2, 2, 16, 16)))
+    pos, freq = torch.rand(2, 700, 1, device="cuda", generator=gen) * 9, sequence.rotary_frequencies((8,))
+    lengths = torch.tensor([700, 333], dtype=torch.int32, device="cuda")
+
+    def run(unpack):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v, w, -g, S)]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            a, b = sequence.head_norm_rotary(leaves[0], leaves[1], pos, freq, (8,), leaves[3], leaves[3])
+            o, last = sequence.decay_attention(a, b, leaves[2], leaves[4], state=leaves[5], lengths=lengths)
+        return torch.autograd.grad((o, last), leaves, (o.detach(), last.detach()))
+    want = run(lambda t: t)
+    for unpack in (spread, at_odd_place, lambda t: spread(t.clone())):
+        assert all(torch.equal(x, y) for x, y in zip(want, run(unpack)))
+    for unpack in (lambda t: t.half() if t.is_floating_point() else t, lambda t: t[..., :8], lambda t: t.cpu()):
+        with pytest.raises(RuntimeError, match="saved tensor"):
+            run(unpack)
