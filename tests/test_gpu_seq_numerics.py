@@ -41,3 +41,37 @@ def test_16_bit_results_are_32_bit_ones_rounded(dtype, dims):
         y = y.detach().to(dtype).double()
         rel = ((x.detach().cpu().double() - y).norm() / y.norm()).item()
         assert rel <= (2 * ref.FP32 / 4 * u) ** 0.5, (name, rel)
+
+
+def recurrence(k, v, g, state):
+    """The states after each token in float64: k, v [B, T, H, D]."""
+    lam = torch.exp(g.double())[:, None, None]
+    for t in range(k.shape[1]):
+        state = lam * state + k[:, t].double().unsqueeze(-1) * v[:, t].double().unsqueeze(-2)
+        yield state
+
+
+@pytest.mark.parametrize("pool", [False, True])
+def test_single_tokens_add_up_to_the_sequence(pool):
+    """6000 single tokens, heads that remember a few to a hundred thousand of
+    them. Every token rounds a state twice, by up to 2^-24 of it and to either
+    side: over the horizon of 1 / |g| tokens (6000 at most) that is 2^-23 of its
+    root. (A decay that is off by the same 2^-25 at each of them would be
+    horizon times that: 1.8e-4 for 6000.)"""
+    from flash_cqt import sequence
+    T, H, D = 6000, 5, 16
+    gen = torch.Generator().manual_seed(61)
+    q, k, v = (randn(gen, 1, T, H, D).cuda() + 0.3 for _ in range(3))
+    g = -torch.tensor([0.7, 0.3, 2.0 ** -10.5, 1e-4, 1e-5], device="cuda")
+    S = torch.zeros(3 if pool else 1, H, D, D, device="cuda")
+    slots = torch.tensor([2], dtype=torch.int32, device="cuda") if pool else None
+    for t in range(T):
+        o = sequence.decay_attention_step(q[:, t], k[:, t], v[:, t], g, S, slots=slots)
+    for want in recurrence(k, v, g, torch.zeros(1, H, D, D, device="cuda", dtype=torch.float64)):
+        pass
+    whole, last = sequence.decay_attention(q, k, v, g)
+    bound = 2.0 ** -23 * (1 / g.abs().double()).clamp(max=T).sqrt() + ref.FP32
+    for got in (S[-1:], last):
+        far = (got.double() - want).flatten(2).norm(dim=2)[0] / want.flatten(2).norm(dim=2)[0]
+        assert (far <= bound).all(), (far, bound)
+    ref.close(o, torch.matmul(q[:, -1].double().unsqueeze(2), want).squeeze(2) / 4, slack=6)
