@@ -76,7 +76,9 @@ __global__ __launch_bounds__(kThreads) void k_scan(Scan a) {
             const int j = j0 + i, s = a.back ? a.segments - 1 - j : j;
             if (j < a.segments) {
                 U[s * step] = x;
-                x = power(g, int(max(min(a.segment, length - s * a.segment), int64_t(0)))) * x + u[i];
+                const Decay f(g, int(max(min(a.segment, length - s * a.segment), int64_t(0))));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(f.by, x[e], f.slow ? x[e] : 0.0f) + u[i][e];
             }
         }
     }

@@ -176,6 +176,15 @@ __device__ __forceinline__ float power(float g, int n) {
     return fabsf(x) < 100.0f ? fmaf(y, fmaf(g, float(n), -x), y) : y;
 }
 
+// What n tokens make of a state that goes on: near one L^n itself, rounded, would be off by the same amount at every chunk,
+// segment or call of as many tokens, which adds up over a head's horizon (6000 calls of one token, g = -1e-4: 6e-5 of the
+// state), so L^n x is x + expm1(g n) x in one rounding there.
+struct Decay {
+    bool slow;
+    float by;                       // expm1(g n) or, for large n, L^n
+    __device__ __forceinline__ Decay(float g, int n) : slow(g * float(n) > -0.5f), by(slow ? expm1f(g * float(n)) : power(g, n)) {}
+};
+
 // kStates: states alone, no output. kSlope: with the slope's terms (1 of dq, 2 of dk). Its registers are shared among two
 // waves of a SIMD.
 template <class T, int KD, int NW, bool kStates, int kSlope>
@@ -216,14 +225,6 @@ __global__ __launch_bounds__(64 * NW, 2) void k_chunks(Chunks a) {
         near[x] = n < 0 ? 0.0f : a.p_scale * power(g, n);
         if (x < C) ahead[x] = a.x_scale * power(g, x + shift);
     }
-
-    // A whole chunk's decay, as two floats, and how far the state has been decayed too little by the factors used so far
-    // (in units of one factor): its rounding, the same in every chunk, would add up over a head's horizon, so a chunk's
-    // factor makes good what those before left. (8 x 7680 fp32 over eight sets of inputs: the decays' gradient is 3.6e-7
-    // of itself off instead of 4.6e-7, those of q, k and v 4.4e-7 instead of 4.6e-7, in the same time; ragged rows 1% more.)
-    const double decay = exp(double(g) * C);
-    const float decay_high = uniform(float(decay)), decay_low = uniform(isfinite(float(decay)) ? float(decay - double(float(decay))) : 0.0f);
-    float owed = 0;
 
     f32x16 S[MT];
     // Addresses are a uniform base and a 32-bit offset of the lane's (the host checks that a chunk's rows and a state
@@ -357,7 +358,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_chunks(Chunks a) {
     const bool fits = a.kd == KD && a.vd == 32 * NW;  // no columns that are not there
     f32x16 O[kStates ? 1 : IT];                                      // transposed: rows the columns of v, columns the queries
     double slopes = 0;                                               // (terms of both signs, far larger than their sum)
-    int before = -1;                                                 // the n that `left` was made for
+    int before = -1;                                                 // the n that `left` and the next two were made for
+    float by = 0, same = 0;                                          // Decay: what the state gets and keeps of itself
     const int chunks = int((a.tokens + C - 1) / C);
     auto flow_at = [&](int64_t c0) {                                 // this wave's part of a chunk's state
         // (a count of pieces of 8 KB and more)
@@ -391,6 +393,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_chunks(Chunks a) {
                 const int m = n - shift - x;
                 left[x] = m < 0 ? 0.0f : a.u_scale * power(g, m);
             }
+            const Decay f(g, n);
+            by = uniform(f.by), same = uniform(f.slow ? 1.0f : 0.0f);
             before = n;
         }
         __syncthreads();
@@ -530,17 +534,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_chunks(Chunks a) {
         if (!kEarly && kSlope == 2) load(ci1, gi1);
         const bool decays = !kStates && (reduce ? first : final), updates = (reduce || kStates || final) && (kStates || a.last.data || step + per < steps);
         if (decays) {
-            float f = power(g, n);
-            if (n == C) {
-                const float rest = owed + decay_low;
-                f = decay_high + rest;
-                owed = uniform(isfinite(f) ? rest - (f - decay_high) : 0.0f);
-            }
-            if constexpr (kSlope == 1) slope += f * float(n) * crossing;
+            if constexpr (kSlope == 1) slope += (by + same) * float(n) * crossing;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) S[m][r] *= f;
+                for (int r = 0; r < 16; ++r) S[m][r] = fmaf(by, S[m][r], same * S[m][r]);
         }
         fence();
 #pragma unroll

@@ -75,3 +75,36 @@ def test_single_tokens_add_up_to_the_sequence(pool):
         far = (got.double() - want).flatten(2).norm(dim=2)[0] / want.flatten(2).norm(dim=2)[0]
         assert (far <= bound).all(), (far, bound)
     ref.close(o, torch.matmul(q[:, -1].double().unsqueeze(2), want).squeeze(2) / 4, slack=6)
+
+
+@pytest.mark.parametrize("n", [1, 3, 64])
+def test_short_calls_add_up_to_the_sequence(n):
+    """The same in calls of n tokens, the state handed on."""
+    from flash_cqt import sequence
+    calls, H, D = (6000 if n < 64 else 1500), 5, 16
+    gen = torch.Generator().manual_seed(67)
+    q, k, v = (randn(gen, 1, calls * n, H, D).cuda() + 0.3 for _ in range(3))
+    g = -torch.tensor([0.7, 0.3, 2.0 ** -10.5, 1e-4, 1e-5], device="cuda") / n
+    state = torch.zeros(1, H, D, D, device="cuda")
+    for t in range(0, calls * n, n):
+        _, state = sequence.decay_attention(*(x[:, t:t + n] for x in (q, k, v)), g, state=state)
+    left = torch.exp(g.double() * torch.arange(calls * n - 1, -1, -1, device="cuda").unsqueeze(-1))
+    want = torch.einsum("th,thi,thj->hij", left, k[0].double(), v[0].double())
+    # what each call adds is itself rounded, to FP32 of it, and n additions or fewer come between two decays
+    bound = 2.0 ** -23 * (1 / g.abs().double()).clamp(max=calls * n).sqrt() + ref.FP32
+    far = (state[0].double() - want).flatten(1).norm(dim=1) / want.flatten(1).norm(dim=1)
+    assert (far <= bound).all(), (far, bound)
+
+
+def test_segments_add_up_to_the_sequence():
+    """One row of 65600 tokens that the GPU walks in many segments, each carried on by the scan."""
+    from flash_cqt import sequence
+    T, H, D = 65600, 3, 16
+    gen = torch.Generator().manual_seed(71)
+    q, k, v = (randn(gen, 1, T, H, D).cuda() + 0.3 for _ in range(3))
+    g = -torch.tensor([1e-3, 2e-5, 1.7e-6], device="cuda")
+    _, last = sequence.decay_attention(q, k, v, g)
+    left = torch.exp(g.double() * torch.arange(T - 1, -1, -1, device="cuda").unsqueeze(-1))
+    want = torch.einsum("th,thi,thj->hij", left, k[0].double(), v[0].double())
+    far = (last[0].double() - want).flatten(1).norm(dim=1) / want.flatten(1).norm(dim=1)
+    assert (far <= 2 * ref.FP32).all(), far
