@@ -47,6 +47,16 @@ def _scale(name, t, like):
     return t.data_ptr()
 
 
+def _clipping(grad_scale, devices):
+    if grad_scale is None:
+        return
+    if not (torch.is_tensor(grad_scale) and grad_scale.is_cuda and grad_scale.numel() == 1 and grad_scale.dtype == torch.float32):
+        raise ValueError("grad_scale must be a float32 tensor of one element on the GPU")
+    for d in devices:
+        if grad_scale.device != d:
+            raise ValueError(f"grad_scale is on {grad_scale.device}, a tensor on {d}")
+
+
 def _factors(step, lr, betas, eps, weight_decay):
     b1, b2 = betas
     if not (step >= 1 and lr >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1 and eps > 0 and weight_decay >= 0):
@@ -96,9 +106,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
     _n.no_tangents(*params, *grads, *exp_avgs, *exp_avg_sqs, grad_scale)
     bits = 32 if lists is None else 8
     state = (torch.float32,) if bits == 32 else (torch.uint8,)
-    if grad_scale is not None and not (torch.is_tensor(grad_scale) and grad_scale.is_cuda and grad_scale.numel() == 1
-                                       and grad_scale.dtype == torch.float32):
-        raise ValueError("grad_scale must be a float32 tensor of one element on the GPU")
+    _clipping(grad_scale, ())
     groups = {}
     for i, p in enumerate(params):
         d = _n.AdamwTensor(_tensor(f"params[{i}]", p, p, _n.DTYPES), _tensor(f"grads[{i}]", grads[i], p, (p.dtype,)),
@@ -107,9 +115,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
                            None if lists is None else _scale(f"scales[0][{i}]", lists[0][i], p),
                            None if lists is None else _scale(f"scales[1][{i}]", lists[1][i], p), p.numel())
         groups.setdefault((p.dtype, p.device), []).append(d)
+    _clipping(grad_scale, {device for _, device in groups})
     for i, ((dtype, device), ds) in enumerate(groups.items()):
-        if grad_scale is not None and grad_scale.device != device:
-            raise ValueError(f"grad_scale is on {grad_scale.device}, a tensor on {device}")
         ts, gs, stream = (_n.AdamwTensor * len(ds))(*ds), _ptr(grad_scale), _n.stream_handle(device.index)
         if bits == 8 and seed is not None:
             status = _n.load().fcqt_adamw_drawn(ts, len(ds), _n.DTYPES[dtype], _n.AdamwFactors(*f), gs,
@@ -168,16 +175,15 @@ class AdamW(torch.optim.Optimizer):
                                       min_8bit=min_8bit, seed=seed))
 
     def _state(self, p, group):
-        s = self.state[p]
+        """The state of p, a new one where it has none (not yet kept)."""
+        s = self.state.get(p)
         if not s:
-            s["step"] = 0
-            if group["state_bits"] == 8 and p.numel() >= group["min_8bit"]:
-                for name in ("exp_avg", "exp_avg_sq"):
-                    s[name] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+            s = {"step": 0}
+            eight = group["state_bits"] == 8 and p.numel() >= group["min_8bit"]
+            for name in ("exp_avg", "exp_avg_sq"):
+                s[name] = torch.zeros(p.shape, dtype=torch.uint8 if eight else torch.float32, device=p.device)
+                if eight:
                     s[name + "_scale"] = torch.zeros(_blocks(p.numel()), dtype=torch.float32, device=p.device)
-            else:
-                for name in ("exp_avg", "exp_avg_sq"):
-                    s[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
         return s
 
     def load_state_dict(self, state_dict):
@@ -204,21 +210,31 @@ class AdamW(torch.optim.Optimizer):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step under stream capture would replay one step's factors; capture adamw_step "
                                "only where that is meant")
+        # all is looked over before anything changes: a call that raises leaves weights, moments and counts as they were
+        calls = []
         for i, group in enumerate(self.param_groups):
             # tensors of one count of steps and one kind of moments go together
             sets = {}
-            for p in group["params"]:
+            for j, p in enumerate(group["params"]):
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
                     raise ValueError("AdamW takes dense gradients")
+                if not (p.is_cuda and p.is_contiguous() and p.dtype in _n.DTYPES):       # (its gradient is alike)
+                    _tensor(f"parameter {j} of group {i}", p, p, _n.DTYPES)
                 s = self._state(p, group)
-                s["step"] += 1
-                sets.setdefault((s["step"], "exp_avg_scale" in s), []).append((p, p.grad.contiguous(), s))
+                sets.setdefault((s["step"] + 1, "exp_avg_scale" in s), []).append((p, p.grad.contiguous(), s))
             for (step, eight), ps in sets.items():
-                scales = tuple([s[n] for _, _, s in ps] for n in ("exp_avg_scale", "exp_avg_sq_scale")) if eight else None
-                adamw_step([p for p, _, _ in ps], [g for _, g, _ in ps], [s["exp_avg"] for _, _, s in ps],
-                           [s["exp_avg_sq"] for _, _, s in ps], step=step, lr=group["lr"], betas=group["betas"],
-                           eps=group["eps"], weight_decay=group["weight_decay"], scales=scales, grad_scale=grad_scale,
-                           seed=group["seed"] + (i << 32))
+                _factors(step, group["lr"], group["betas"], group["eps"], group["weight_decay"])
+                _clipping(grad_scale, {p.device for p, _, _ in ps})
+                calls.append((i, group, step, eight, ps))
+        for i, group, step, eight, ps in calls:
+            scales = tuple([s[n] for _, _, s in ps] for n in ("exp_avg_scale", "exp_avg_sq_scale")) if eight else None
+            adamw_step([p for p, _, _ in ps], [g for _, g, _ in ps], [s["exp_avg"] for _, _, s in ps],
+                       [s["exp_avg_sq"] for _, _, s in ps], step=step, lr=group["lr"], betas=group["betas"],
+                       eps=group["eps"], weight_decay=group["weight_decay"], scales=scales, grad_scale=grad_scale,
+                       seed=group["seed"] + (i << 32))
+            for p, _, s in ps:
+                s["step"] = step
+                self.state[p] = s
         return loss
