@@ -188,7 +188,12 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch.optim's, which casts a state to its parameter's type: codes
-        and scales keep theirs."""
+        and scales keep theirs. One of torch.optim.AdamW's is taken up too, its
+        moments as float32."""
+        for group in state_dict["param_groups"]:
+            for name, other in (("amsgrad", True), ("maximize", True), ("decoupled_weight_decay", False)):
+                if group.get(name) is other:
+                    raise ValueError(f"the state is one of {name}={other}, which this AdamW does not do")
         super().load_state_dict(state_dict)
         for group in self.param_groups:
             for name, x in self.defaults.items():
@@ -198,8 +203,11 @@ class AdamW(torch.optim.Optimizer):
         for i, s in state_dict["state"].items():
             p = index[i]
             for name, x in s.items():
-                if torch.is_tensor(x):
-                    self.state[p][name] = x.detach().clone().to(p.device)
+                if name == "step":
+                    self.state[p][name] = int(x)
+                elif torch.is_tensor(x):
+                    x = x.detach().clone().to(p.device)
+                    self.state[p][name] = x.float().contiguous() if x.is_floating_point() else x
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale=None):

@@ -1,8 +1,11 @@
-"""optim.AdamW's state: a step that is refused changes nothing."""
+"""optim.AdamW's state: a step that is refused changes nothing, and one of
+torch.optim.AdamW's is taken up."""
 import copy
 
 import pytest
 import torch
+
+import seq_ref as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +65,44 @@ def test_a_refused_step_changes_nothing(bits, begun):
     other.step()
     assert all(torch.equal(p, q) for p, q in zip(good, qs))
     assert opt.state[good[0]]["step"] == opt.state[good[1]]["step"] == 1 + begun
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_state_of_torchs_adamw(dtype):
+    """Its steps are tensors and its moments of the parameter's type: taken up as
+    counts and float32, tensors go in one call, and the run goes on by the rule."""
+    from flash_cqt import optim
+    gen = torch.Generator("cuda").manual_seed(2)
+    ps = [torch.nn.Parameter(torch.randn(n, device="cuda", generator=gen).to(dtype)) for n in (40, 7)]
+    how = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+    theirs = torch.optim.AdamW(ps, **how)
+    grads = [[torch.randn(p.shape, device="cuda", generator=gen).to(dtype) for p in ps] for _ in range(3)]
+    for gs in grads[:2]:
+        for p, g in zip(ps, gs):
+            p.grad = g
+        theirs.step()
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    ours = optim.AdamW(qs)
+    ours.load_state_dict(theirs.state_dict())
+    assert ours.param_groups[0]["lr"] == 1e-2 and ours.param_groups[0]["state_bits"] == 32
+    calls = []
+    step, optim.adamw_step = optim.adamw_step, lambda *a, **k: (calls.append(len(a[0])), step(*a, **k))
+    try:
+        for q, g in zip(qs, grads[2]):
+            q.grad = g
+        ours.step()
+    finally:
+        optim.adamw_step = step
+    assert calls == [2] and all(ours.state[q]["step"] == 3 for q in qs)
+    for p, q, g in zip(ps, qs, grads[2]):
+        s = theirs.state[p]
+        want = ref.adamw(p.detach().cpu().double(), g.cpu().double(), s["exp_avg"].cpu().double(), s["exp_avg_sq"].cpu().double(), step=3, **how)
+        for x, y, t in zip((q, ours.state[q]["exp_avg"], ours.state[q]["exp_avg_sq"]), want, (dtype, torch.float32, torch.float32)):
+            ref.close(x, y, t)
+    for kw in (dict(amsgrad=True), dict(maximize=True)):
+        before = copy.deepcopy(ours.state_dict())
+        with pytest.raises(ValueError, match="does not do"):
+            ours.load_state_dict(torch.optim.AdamW(ps, **kw).state_dict())
+        assert same(ours.state_dict(), before)
+    with pytest.raises(ValueError, match="decoupled"):
+        ours.load_state_dict(torch.optim.Adam(ps).state_dict())
