@@ -170,10 +170,10 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Tensors a, fcqt_adamw_factor
                              reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
     if (left >= V && (places & 15) == 0) {
         float pp[V], gg[V], mm[V], vv[V], w;
-        load<T, V>(p, true, pp);
-        load<T, V>(g, true, gg);
-        load<float, V>(m, true, mm);
-        load<float, V>(v, true, vv);
+        load<T, V>(p, pp);
+        load<T, V>(g, gg);
+        load<float, V>(m, mm);
+        load<float, V>(v, vv);
 #pragma unroll
         for (int e = 0; e < V; ++e) pp[e] = updated(pp[e], grad_scale ? gg[e] * gs : gg[e], mm[e], vv[e], w, f);
         store<T, V>(p, pp);
@@ -214,8 +214,8 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(Tensors a, fcqt_adamw_facto
         vs = t.v_scale[at / kBlock];
     }
     if (wide) {
-        load<T, V>(p, true, pp);
-        load<T, V>(g, true, gg);
+        load<T, V>(p, pp);
+        load<T, V>(g, gg);
         const Pack<uint8_t, V> x = *reinterpret_cast<Pack<uint8_t, V>*>(m), y = *reinterpret_cast<Pack<uint8_t, V>*>(v);
 #pragma unroll
         for (int e = 0; e < V; ++e) mc[e] = x.e[e], vc[e] = y.e[e];

@@ -132,7 +132,7 @@ struct Shape {
     int32_t dtype;
 };
 
-int checked(const fcqt_heads* s, int elem, int64_t batch, int64_t tokens) {
+int checked(const fcqt_heads* s, int elem) {
     if (!s || !s->data || s->heads < 1 || s->heads > 65535) return FCQT_EARG;
     // rows are read 16 bytes at a time, and a chunk's with offsets of 32 bits
     if (!aligned(s->data, 16) || ((s->batch_stride | s->token_stride | s->head_stride) * elem) % 16) return FCQT_EALIGN;
@@ -225,7 +225,7 @@ extern "C" int fcqt_decay_attention(const fcqt_heads* q, const fcqt_heads* k, co
     if (!aligned(log_decay, 4) || !aligned(lengths, 4) || !aligned(state, 16) || !aligned(last, 16)) return FCQT_EALIGN;
     if (!tokens) return copy_state(state, last, batch * s.hk * dk * dv, stream);
     for (const fcqt_heads* x : {q, k, v})
-        if (int e = checked(x, size_of(dtype), batch, tokens)) return e;
+        if (int e = checked(x, size_of(dtype))) return e;
     if (!o) return FCQT_EARG;
     if (!aligned(o, 16) || !aligned(workspace, 16)) return FCQT_EALIGN;
     if (workspace_bytes < fcqt_decay_attention_workspace(batch, tokens, s.hq, s.hk, dk, dv, dtype, lengths != nullptr, 0)) return FCQT_EARG;
@@ -269,7 +269,7 @@ extern "C" int fcqt_decay_attention_bwd(const fcqt_heads* q, const fcqt_heads* k
         return copy_state(glast, dstate, all, stream);
     }
     for (const fcqt_heads* x : {q, k, v, go})
-        if (int e = checked(x, size_of(dtype), batch, tokens)) return e;
+        if (int e = checked(x, size_of(dtype))) return e;
     const bool slope = dlog_decay != nullptr;
     const int64_t need = fcqt_decay_attention_workspace(batch, tokens, s.hq, s.hk, dk, dv, dtype, lengths != nullptr, slope ? 2 : 1);
     if (!dq || !dk_ || !dv_ || workspace_bytes < need || (need && !workspace)) return FCQT_EARG;

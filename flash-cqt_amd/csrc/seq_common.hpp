@@ -46,21 +46,15 @@ __device__ __forceinline__ bf16 narrow(float x) { return {__builtin_bit_cast(uin
 template <>
 __device__ __forceinline__ f16 narrow(float x) { return {__builtin_bit_cast(uint16_t, static_cast<_Float16>(x))}; }
 
-// V consecutive elements as one load or store where their place allows it (wide), else one by one
+// V consecutive elements as one load or store
 template <class T, int V>
 struct alignas(sizeof(T) * V) Pack {
     T e[V];
 };
 
 template <class T, int V>
-__device__ __forceinline__ void load(const T* p, bool wide, float (&x)[V]) {
-    Pack<T, V> a;
-    if (wide) {
-        a = *reinterpret_cast<const Pack<T, V>*>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) a.e[i] = p[i];
-    }
+__device__ __forceinline__ void load(const T* p, float (&x)[V]) {
+    const Pack<T, V> a = *reinterpret_cast<const Pack<T, V>*>(p);
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] = widen<T>(a.e[i]);
 }

@@ -321,7 +321,7 @@ bool placed(const fcqt_heads& s, int bytes, int elem) {
     return aligned(s.data, bytes) && ((s.batch_stride | s.token_stride | s.head_stride) * elem) % bytes == 0;
 }
 
-int checked(const fcqt_heads* s, int64_t batch, int64_t tokens, int elem) {
+int checked(const fcqt_heads* s, int elem) {
     if (!s || s->heads < 1 || s->heads > 65536 || !s->data) return FCQT_EARG;
     return aligned(s->data, elem) ? FCQT_OK : FCQT_EALIGN;
 }
@@ -398,8 +398,8 @@ extern "C" int fcqt_head_norm_rotary(const fcqt_heads* q, const fcqt_heads* k, c
     Args a{};
     if (int e = prepare(a, rot, batch, tokens, dim, dtype)) return e;
     if (a.all == 0) return FCQT_OK;
-    if (int e = checked(q, batch, tokens, size_of(dtype))) return e;
-    if (int e = checked(k, batch, tokens, size_of(dtype))) return e;
+    if (int e = checked(q, size_of(dtype))) return e;
+    if (int e = checked(k, size_of(dtype))) return e;
     if (!q_out || !k_out) return FCQT_EARG;
     if (!aligned(wq, 4) || !aligned(wk, 4)) return FCQT_EALIGN;
     a.q = *q, a.k = *k, a.wq = wq, a.wk = wk, a.oq = q_out, a.ok = k_out, a.norm = norm, a.eps = eps;
@@ -409,7 +409,8 @@ extern "C" int fcqt_head_norm_rotary(const fcqt_heads* q, const fcqt_heads* k, c
     return run(a, false, grid, dtype, stream);
 }
 
-extern "C" int64_t fcqt_head_norm_rotary_partial(int64_t batch, int64_t tokens, int32_t heads, int32_t dim, int32_t dtype) {
+// (the same for all shapes but the head dimension)
+extern "C" int64_t fcqt_head_norm_rotary_partial(int64_t, int64_t, int32_t, int32_t dim, int32_t) {
     return int64_t(kBackGroups) * 2 * dim;
 }
 
@@ -424,7 +425,7 @@ extern "C" int fcqt_head_norm_rotary_bwd(const fcqt_heads* q, const fcqt_heads* 
     int64_t grid = 0;
     if (a.all) {
         for (const fcqt_heads* s : {q, k, gq, gk})
-            if (int e = checked(s, batch, tokens, size_of(dtype))) return e;
+            if (int e = checked(s, size_of(dtype))) return e;
         if (!dq || !dk || q->heads != gq->heads || k->heads != gk->heads) return FCQT_EARG;
         a.q = *q, a.k = *k, a.gq = *gq, a.gk = *gk, a.wq = wq, a.wk = wk, a.oq = dq, a.ok = dk, a.norm = norm, a.eps = eps;
         a.partial = partial;

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(kThreads) void k_step(Args a) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const int r = rl + i * kLanes;
-        if (in && r < a.dk) load<float, 4>(s + int64_t(r) * a.dv, true, x[i]);
+        if (in && r < a.dk) load<float, 4>(s + int64_t(r) * a.dv, x[i]);
     }
     for (int i = threadIdx.x; i < a.dk; i += kThreads) ks[i] = element<T>(a.k, row, head, i);
     float v[4] = {};
