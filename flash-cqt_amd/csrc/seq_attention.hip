@@ -25,7 +25,7 @@ int padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
 // A kernel with inner dimension kd (padded) and vd columns, 32 a wave, over `tokens` tokens cut into segments of `segment`.
 // Two waves where they hold all columns (for 128, twice two would load q and k again: 8 x 7680 bf16 tokens of 8 heads with
-// gradients 1446 us, four waves 1023).
+// gradients 1446 us, four waves 1023, both with operands of 16 bits).
 Plan sized(int kd, int vd, int64_t tokens, int64_t segment) {
     Plan p;
     p.kd = padded(kd);
@@ -101,8 +101,8 @@ __global__ __launch_bounds__(kThreads) void k_slopes(const double* first, const 
 }
 
 // Whether every query head of a group has a workgroup of its own: where they share one, its state is updated once, but
-// the group's heads are one after the other. 1 x 1958 bf16 tokens, 12 heads on 3, 64 wide: 24 us apart, 41 shared; 8 x 4000,
-// 16 heads on 4, 128 wide: 194 apart, 169 shared.
+// the group's heads are one after the other. 1 x 1958 bf16 tokens, 12 heads on 3, 64 wide: 27 us apart, 48 shared; 8 x 4000,
+// 16 heads on 4, 128 wide: 219 apart, 184 shared.
 bool spreads(const Plan& p, int64_t batch, int keys, int group) {
     return group > 1 && batch * keys * p.segments < 512;
 }
@@ -151,12 +151,12 @@ int shape_of(Shape& s, int64_t batch, int64_t tokens, int32_t hq, int32_t hk, in
 
 // Tokens of a segment, one cut for the outputs and all gradients. Whole rows are cut into as many workgroups as the GPU
 // holds at a time (by the LDS of the main kernels: three on a CU for 16-bit types up to 64 wide, one for fp32 over 64, two
-// otherwise). With gradients, 8 x 7680 tokens of 8 heads: 450 us in 768 workgroups, 569 in 512 (bf16, 64 wide), 2340 us in
-// 256, 2432 in 512 (fp32, 128 wide); 24 x 4096 tokens of 16 heads, bf16, 64 wide: 1389 us in 768, 1970 in 384. Rows with
+// otherwise). With gradients, 8 x 7680 tokens of 8 heads: 450 us in 768 workgroups, 557 in 512 (bf16, 64 wide), 2349 us in
+// 256, 2358 in 512 (fp32, 128 wide); 24 x 4096 tokens of 16 heads, bf16, 64 wide: 1350 us in 768, 1904 in 384. Rows with
 // lengths of their own are cut into 1024: half of them ending early leaves half of the workgroups idle (9 rows of 0 to 4097
-// tokens take 20% less than with 512). A segment costs a state, written, scanned and read, so none is under 64 tokens
-// and the scan's steps stay few beside the chunks that a segment saves: 512 tokens of 64 fp32 heads of 64 take 73 us in
-// one segment, 37 in eight.
+// tokens: 717 us, 821 with 512). A segment costs a state, written, scanned and read, so none is under 64 tokens
+// and the scan's steps stay few beside the chunks that a segment saves: 512 tokens of 64 fp32 heads of 64 take 76 us in
+// one segment, 32 in eight.
 int64_t segment_of(const Shape& s, bool ragged) {
     const int64_t tokens = std::max<int64_t>(s.tokens, 1);
     const int64_t groups = s.batch * s.hk;
@@ -177,7 +177,8 @@ int64_t state_floats(const Shape& s, int64_t segment) {
     return segments > 1 ? s.batch * s.hk * segments * s.dk * s.dv : 0;
 }
 
-// What the backward pass keeps, in floats: the states that segments start from, both ways; where the decays' gradient
+// What the backward pass keeps, in floats: the states that segments start from, both ways (forwards only without those of
+// the forward pass); where the decays' gradient
 // is wanted, the state's gradient at every chunk's end and the sums.
 struct Parts {
     int64_t states, flow, slopes;

@@ -27,13 +27,15 @@
 // v_mfma_f32_32x32x2_f32 takes 512. (Two planes for what 16-bit outputs are made of would leave 2^-17 of each operand, and
 // o 1.3e-6 of its size away from its value before the rounding, where three leave 2e-7.)
 //
-// What bounds it: 1 x 65537 bf16 tokens of 16 heads, 128 wide, take 290 us in the main kernel (1.07 GB, 3.7 TB/s; its
-// loads alone 182 us, its instructions alone 290) after 127 us for the segments' own states (0.54 GB, 4.2 TB/s): about
-// 1000 vector and 100 matrix instructions a wave and chunk, two waves a SIMD, whose registers the state fills. A pass of
-// one segment would need no states first, but 16 workgroups leave 240 compute units idle. 8 x 512 fp32 tokens of 8 heads of
-// 64: 15 us, 12 for the states, 5 between them, each little more than its launch and one chunk after the other. dq's
-// kernel with the slope's terms takes 197 us for 9 rows of 0 to 4097 tokens, 16 heads on 8 (dq alone 95, dk with its half
-// of the terms 151): most of the difference is the states at the chunks' ends, 64 KB for 64 tokens of a head.
+// What bounds it: 1 x 65537 bf16 tokens of 16 heads, 128 wide, take 373 us in the main kernel (1.11 GB, 3.0 TB/s) after
+// 128 us for the segments' own states (0.54 GB, 4.2 TB/s): about 1600 vector and 136 matrix instructions a wave and chunk,
+// 169 and 117 us of the SIMDs' time; the rest is waiting for LDS, barriers and products that need each other, which two
+// waves a SIMD (their registers are full of state) cover in part. Every wave computes all of P, whose rows its columns of v
+// need. A pass of one segment would need no states first, but 16 workgroups leave 240 compute units idle. 8 x 512 fp32
+// tokens of 8 heads of 64: 15 us, 12 for the states, 5 between them, each little more than its launch and one chunk after
+// the other. dq's kernel with the slope's terms takes 198 us for 9 rows of 0 to 4097 tokens, 16 heads on 8 (dq alone 115, dk
+// with its half of the terms 158): most of the difference is the states at the chunks' ends, 64 KB for 64 tokens of a head.
+// fp16's two planes and 32-token chunks take 573 us where bf16 takes 373.
 // Chunks of 64 tokens, or of 32 where planes take the LDS: at 32 tokens bf16 would read twice as many of those.
 #pragma once
 

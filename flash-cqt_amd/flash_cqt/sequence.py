@@ -7,7 +7,8 @@ at a time beside TrainableCQT and SlicedCQT.
     o = decay_attention_step(q, k, v, log_decay, states, slots=slots)
 
 Tensors are float32, bfloat16 or float16 on one GPU; sums, norms and states
-are float32. head_norm_rotary and decay_attention record gradients. Work goes
+are float32. head_norm_rotary and decay_attention record gradients (tangents
+of forward mode raise). Work goes
 to the current stream of the tensors' device, which must be the current one.
 Strided inputs are read in place where their last dimension is contiguous.
 """
@@ -112,7 +113,8 @@ def head_norm_rotary(q, k, positions=None, freq=None, sections=(), wq=None, wk=N
     the A axes turns, in order. The angle is the float32 product of the two.
     Pairs are (j, j + sum(sections)) or, interleaved, (2j, 2j + 1); elements
     past the last pair stay. positions=None: no rotation; norm=False: rotation
-    alone. Gradients go to q, k, wq and wk."""
+    alone. Gradients go to q, k, wq and wk; positions and freq are needed for
+    them, so neither may be changed in place before the backward pass."""
     glue = _glue()
     if glue is not None and _plain(q, k, positions, freq, wq, wk):
         out = glue.norm_rotary(q, k, positions, freq, sections, wq, wk, eps, interleaved, norm)
@@ -238,8 +240,9 @@ def decay_attention(q, k, v, log_decay, *, scale=None, state=None, lengths=None)
     valid tokens of each row (None: all); what lies past them may be anything,
     o is zero there and the last state is the one at the length. Gradients go
     to q, k, v, log_decay and state. Dk and Dv are at most 128. The sequence
-    is computed in chunks of up to 64 tokens: a value that is not finite also
-    reaches the tokens before it in its chunk."""
+    is computed in chunks of up to 64 tokens: a value that is not finite, or
+    over bfloat16's largest (3.38e38), makes NaN, in the tokens before it in
+    its chunk too."""
     glue = _glue()
     if glue is not None and _plain(q, k, v, log_decay, state, lengths):
         out = glue.attention(q, k, v, log_decay, state, lengths, scale)
@@ -334,7 +337,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, slots=None, scale=None):
     q [B, Hq, Dk], k [B, Hk, Dk], v [B, Hk, Dv]; Hq is a multiple of Hk, and
     Hq / Hk neighbouring query heads share a key head. log_decay: float32
     [Hk], zero or below; scale: Dk ** -0.5 unless given. state: float32
-    [pool, Hk, Dk, Dv], contiguous. slots: int32 [B], the state of each row,
+    [pool, Hk, Dk, Dv], contiguous, at a multiple of 16 bytes. slots: int32
+    [B], the state of each row,
     without repeats, or None: row b has state b. A row whose slot is outside
     the pool (-1, say) has no sequence: its o is zero and no state changes.
     No gradients: decay_attention records them, over whole sequences."""

@@ -80,8 +80,9 @@ int fcqt_head_norm_rotary_bwd(const fcqt_heads* q, const fcqt_heads* k, const fc
  * (NULL: all; taken into 0..tokens); what lies past them is not used, o is zero there and `last` is the state at the
  * length. o: contiguous [batch][tokens][hq][dv]. q, k and v are read 16 bytes at a time: their places and strides are
  * multiples of that, token strides under 2^31 bytes / 64. dk and dv are multiples of 8, at most
- * FCQT_DECAY_MAX_DIM; batch at most 65535, tokens below 2^31 - 64. workspace: fcqt_decay_attention_workspace(...) bytes (0: NULL will do),
- * ragged where lengths are given, with backward 0; for the gradients with 1, or with 2 where dlog_decay is among them. */
+ * FCQT_DECAY_MAX_DIM; batch at most 65535, tokens below 2^31 - 64. fp32 operands and states go through bf16 planes: a value
+ * over bf16's largest, 3.38e38, or an infinite one makes NaN. workspace: fcqt_decay_attention_workspace(...) bytes (0: NULL
+ * will do), ragged where lengths are given, with backward 0; for the gradients with 1, or with 2 where dlog_decay is among them. */
 int64_t fcqt_decay_attention_workspace(int64_t batch, int64_t tokens, int32_t hq, int32_t hk, int32_t dk, int32_t dv,
                                        int32_t dtype, int32_t ragged, int32_t backward);
 int fcqt_decay_attention(const fcqt_heads* q, const fcqt_heads* k, const fcqt_heads* v, const float* log_decay,
