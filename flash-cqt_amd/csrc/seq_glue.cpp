@@ -1,7 +1,7 @@
 // Host glue of flash_cqt.sequence and flash_cqt.optim for ordinary calls: arguments, outputs, autograd nodes and the
 // launch in one C++ call (host code only; the kernels are libflashcqt_seq.so's, reached through the C ABI function
 // pointers that Python passes in). A token's attention takes 3 us on the GPU and 6 us a call from here, 23 us from
-// Python; a small training pass 80 us against 160. Every function returns None for a call that is not plain (another
+// Python; a small training pass 62 to 68 us against 150. Every function returns None for a call that is not plain (another
 // type or device, tensor subclasses, function or dispatch modes, functorch, tracing, tangents, arguments that do not
 // fit): the Python path, which has the same results, then takes it, or says what is wrong with it.
 #include <cmath>
