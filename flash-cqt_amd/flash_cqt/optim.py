@@ -159,9 +159,9 @@ def read_moments(exp_avgs, exp_avg_sqs, scales, *, out=None):
 
 class AdamW(torch.optim.Optimizer):
     """torch.optim's interface over adamw_step: parameter groups, schedulers,
-    state_dict; parameters are contiguous. state_bits: 32, or 8 for one byte a moment (decided when a
-    parameter first steps; tensors under min_8bit elements keep 32 bits).
-    seed: of the draws that 8-bit moments are rounded by (adamw_step); runs of
+    state_dict; parameters are contiguous. state_bits: 32, or 8 for one byte a
+    moment (decided when a parameter first steps; tensors under min_8bit
+    elements keep 32 bits). seed: of the draws that 8-bit moments are rounded by (adamw_step); runs of
     one seed and the same gradients are the same."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit=4096,
